@@ -69,6 +69,33 @@ class PeerGroup(ctypes.Structure):
     ]
 
 
+_i32, _i64 = ctypes.c_int32, ctypes.c_int64
+
+
+class RotaryProblem(ctypes.Structure):
+    """Mirror of ``struct fbla_rotary_problem``."""
+    _fields_ = [(n, _i32) for n in ("dtype", "batch", "heads_q", "heads_k", "dim", "pairs", "axes", "interleaved",
+                                    "inverse", "positions32", "num_seqs")]
+    _fields_ += [("factor", ctypes.c_float), ("seq_len", _i64), ("offset", _i64)]
+    _fields_ += [(n, _i64 * 3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")]
+    _fields_ += [("pos_stride", _i64 * 2), ("positions", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+                 ("freqs", ctypes.c_void_p)]
+
+
+class ConvProblem(ctypes.Structure):
+    """Mirror of ``struct fbla_conv_problem``."""
+    _fields_ = [(n, _i32) for n in ("dtype", "weight_dtype", "batch", "channels", "width", "silu", "num_seqs", "reserved")]
+    _fields_ += [("seq_len", _i64), ("x_stride", _i64 * 2), ("dy_stride", _i64 * 2), ("cu_seqlens", ctypes.c_void_p)]
+
+
+class ScanProblem(ctypes.Structure):
+    """Mirror of ``struct fbla_scan_problem``."""
+    _fields_ = [(n, _i32) for n in ("dtype", "batch", "channels", "states", "groups", "softplus", "num_seqs", "reserved")]
+    _fields_ += [("seq_len", _i64)]
+    _fields_ += [(n, _i64 * 2) for n in ("x_stride", "dt_stride", "z_stride", "dy_stride")]
+    _fields_ += [("b_stride", _i64 * 3), ("c_stride", _i64 * 3), ("cu_seqlens", ctypes.c_void_p)]
+
+
 _P = ctypes.POINTER(Problem)
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
@@ -88,6 +115,20 @@ _DECOUPLED_SIGNATURES = {
 }
 OPS = ("linear_attn", "simple_la", "decoupled_la", "varlen_linear_attn")
 
+# name -> (problem struct, argument types after the pointer to it, result type)
+_SEQ_SIGNATURES = {
+    "fbla_rotary": (RotaryProblem, [_vp] * 5, ctypes.c_int),                               # q, k, q_out, k_out, stream
+    "fbla_causal_conv_workspace_bytes": (ConvProblem, [], _i64),
+    "fbla_causal_conv_fwd": (ConvProblem, [_vp] * 7, ctypes.c_int),                        # 6 tensors, stream
+    "fbla_causal_conv_bwd": (ConvProblem, [_vp] * 11 + [_sz, _vp], ctypes.c_int),          # 10 tensors, ws, its size, stream
+    "fbla_causal_conv_step": (ConvProblem, [_vp] * 6, ctypes.c_int),                       # 5 tensors, stream
+    "fbla_selective_scan_checkpoint_floats": (ScanProblem, [], _i64),
+    "fbla_selective_scan_workspace_bytes": (ScanProblem, [ctypes.c_int], _i64),
+    "fbla_selective_scan_fwd": (ScanProblem, [_vp] * 13 + [_sz, _vp], ctypes.c_int),       # 12 tensors, ws, its size, stream
+    "fbla_selective_scan_bwd": (ScanProblem, [_vp] * 22 + [_sz, _vp], ctypes.c_int),       # 21 tensors, ws, its size, stream
+    "fbla_selective_scan_step": (ScanProblem, [_vp] * 11, ctypes.c_int),                   # 10 tensors, stream
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -105,6 +146,7 @@ def exported_symbols():
     names += ["fbla_peer_state_sum", "fbla_seq_sharded_supported", "fbla_seq_sharded_part_floats",
               "fbla_seq_sharded_fwd_state", "fbla_seq_sharded_bwd_state", "fbla_seq_sharded_exchange",
               "fbla_device_status", "fbla_clear_device_status", "fbla_unreduced_state"]
+    names += list(_SEQ_SIGNATURES)
     return names
 
 
@@ -179,6 +221,10 @@ def lib():
         L.fbla_pisa_bwd_scratch_floats.argtypes = [_PP]
         L.fbla_pisa_bwd.restype = ctypes.c_int
         L.fbla_pisa_bwd.argtypes = [_PP] + [_vp] * 14 + [_sz, _vp]   # 14 tensors, scratch size, stream
+        for name, (struct, args, res) in _SEQ_SIGNATURES.items():
+            f = getattr(L, name)
+            f.restype = res
+            f.argtypes = [ctypes.POINTER(struct)] + args
         _lib = L
     return _lib
 

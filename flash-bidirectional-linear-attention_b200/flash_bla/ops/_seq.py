@@ -1,0 +1,63 @@
+"""Host-side helpers of the sequence operators beside the attention passes (rotary positions, the
+short causal convolution, the selective scan)."""
+import ctypes
+
+import torch
+
+from flash_bla import _C
+
+FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def require_cuda(x):
+    if not x.is_cuda:
+        raise RuntimeError("flash_bla operators run on CUDA tensors only (there is no CPU path)")
+
+
+def same_device(x, **others):
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the first tensor on {x.device}")
+
+
+def check_cu_seqlens(cu):
+    if not isinstance(cu, torch.Tensor) or cu.ndim != 1 or cu.numel() < 2 or cu.dtype != torch.int32:
+        raise ValueError("cu_seqlens must be an int32 tensor of shape (num_sequences + 1,)")
+    return cu.contiguous()
+
+
+def rows(t):
+    """The tensor with its last dimension contiguous; the others may have any stride."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def stride(t, dim):
+    """Stride that the kernels see: a dimension of one element is never stepped over."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def aligned(t):
+    """States are read 16 bytes at a time: a view at an odd offset is copied."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def refuse_grad(what, *tensors):
+    if wants_grad(*tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def call(fn, prob, like, *args):
+    """One library call on the current stream of ``like``'s device."""
+    with _C.device_guard(like):
+        _C.check(fn(ctypes.byref(prob), *args, _C.stream_of(like)))
+
+
+def scratch(nbytes, like):
+    """(tensor or None, bytes) from torch's caching allocator: a workspace of this call alone."""
+    if nbytes < 0:
+        _C.check(1)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None), nbytes

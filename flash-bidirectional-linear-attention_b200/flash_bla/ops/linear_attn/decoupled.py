@@ -13,6 +13,7 @@ import torch
 
 from flash_bla.ops import _passes as P
 from flash_bla import _C
+from flash_bla.ops.rotary.fused import rotary_embedding
 from flash_bla.utils import contiguous
 
 _OP = "decoupled_la"
@@ -94,3 +95,23 @@ def decoupled_la(
         o = DecoupledLAFunction.apply(*(P.pad_last(x, 64) for x in (q, k, q_rope, k_rope, v)), scale, eps)
         return o[..., :v.shape[-1]]
     return DecoupledLAFunction.apply(q, k, q_rope, k_rope, v, scale, eps)
+
+
+def rotary_decoupled_la(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    freqs: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    *,
+    factor: float = 1.0,
+    interleaved: bool = True,
+    axes: int = 1,
+    scale: Optional[float] = None,
+    eps: float = 1e-6,
+) -> torch.Tensor:
+    r"""`decoupled_la` with `q_rope`, `k_rope` made by `rotary_embedding` from `q`, `k` `(B, H, L, K)` (one
+    kernel, no torch passes in between); `freqs`, `positions`, `factor`, `interleaved` and `axes` as there,
+    `v`, `scale` and `eps` as in `decoupled_la`."""
+    q_rope, k_rope = rotary_embedding(q, k, freqs, positions, factor=factor, interleaved=interleaved, axes=axes)
+    return decoupled_la(q, k, q_rope, k_rope, v, scale, eps)

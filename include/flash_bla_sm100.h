@@ -345,6 +345,128 @@ int fbla_seq_sharded_bwd_state(const fbla_problem *p, const void *q, const void 
 int fbla_seq_sharded_exchange(const fbla_problem *p, const fbla_peer_group *group, float *state_out,
                               fbla_stream_t stream);
 
+/* ---- rotary positions ------------------------------------------------------------------
+ * Turns pairs of features of q and k by an angle that grows with the position -- what
+ * decoupled_la takes as q_rope, k_rope:
+ *   (x0, x1) -> factor * (x0 cos a - x1 sin a, x0 sin a + x1 cos a),  a = position * freqs[pair]
+ * The first 2*pairs of dim features take part; interleaved: features (2i, 2i+1) are pair i, else
+ * (i, i + pairs).  The rest is copied.  inverse = 1 turns by -a: the gradient of the call.
+ * axes > 1: positions carry that many coordinates (contiguous), pair i uses coordinate
+ * i / (pairs / axes).  positions NULL: token index (packed: index in its sequence) + offset.
+ * Strides in elements, in the order batch, head, token; the features are contiguous.  Packed
+ * sequences: batch 1, seq_len = total tokens; tokens that no sequence owns come out as zeros.
+ * The angle is formed and reduced in 64 bits.  No counterpart in the reference (its layers
+ * rotate in torch, flash_bla/layers/mlla.py and rala.py).                                     */
+typedef struct fbla_rotary_problem {
+    int32_t dtype;          /* enum fbla_dtype of q, k and the outputs                  */
+    int32_t batch;
+    int32_t heads_q;
+    int32_t heads_k;        /* 0: no k                                                  */
+    int32_t dim;            /* features per head                                        */
+    int32_t pairs;          /* rotated pairs, 2 * pairs <= dim                          */
+    int32_t axes;           /* coordinates per position; divides pairs                  */
+    int32_t interleaved;
+    int32_t inverse;
+    int32_t positions32;    /* positions are int32, else int64                          */
+    int32_t num_seqs;       /* packed only                                              */
+    float factor;           /* on the rotated features                                  */
+    int64_t seq_len;
+    int64_t offset;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+    int64_t pos_stride[2];  /* batch, token                                             */
+    const void *positions;
+    const int32_t *cu_seqlens; /* device int32 [num_seqs + 1]; NULL: fixed length       */
+    const double *freqs;    /* device, [pairs], radians per position                    */
+} fbla_rotary_problem;
+
+int fbla_rotary(const fbla_rotary_problem *p, const void *q, const void *k, void *q_out,
+                void *k_out, fbla_stream_t stream);
+
+/* ---- short causal convolution ------------------------------------------------------------
+ *   p[t,c] = bias[c] + sum_j w[c,j] x[t-width+1+j, c],   y = p, or p * sigmoid(p) with silu
+ * x, dy: (batch, seq_len, channels) with the given batch and token strides (elements); y, dx
+ * contiguous; w (channels, width), bias (channels) or NULL, both of weight_dtype (fp32 or the type
+ * of x), their gradients too.  States (sequences, width - 1, channels): the last width - 1 inputs,
+ * oldest first; initial_state NULL: zeros; final_state, d_final_state may be NULL.  Packed
+ * sequences: batch 1, cu_seqlens; tokens that no sequence owns come out as zeros, so do their
+ * gradients.  No call uses atomics: the same bits on every run.  No counterpart in the reference. */
+typedef struct fbla_conv_problem {
+    int32_t dtype;
+    int32_t weight_dtype;
+    int32_t batch;          /* at most 65535                                            */
+    int32_t channels;
+    int32_t width;          /* taps, 2..4                                               */
+    int32_t silu;
+    int32_t num_seqs;       /* packed only, at most 65535                               */
+    int32_t reserved;
+    int64_t seq_len;
+    int64_t x_stride[2];    /* batch, token                                             */
+    int64_t dy_stride[2];
+    const int32_t *cu_seqlens;
+} fbla_conv_problem;
+
+/* Bytes of scratch fbla_causal_conv_bwd needs; <0 on error. */
+int64_t fbla_causal_conv_workspace_bytes(const fbla_conv_problem *p);
+int fbla_causal_conv_fwd(const fbla_conv_problem *p, const void *x, const void *w, const void *bias,
+                         const void *initial_state, void *y, void *final_state, fbla_stream_t stream);
+int fbla_causal_conv_bwd(const fbla_conv_problem *p, const void *x, const void *w, const void *bias,
+                         const void *initial_state, const void *dy, const void *d_final_state,
+                         void *dx, void *dw, void *dbias, void *d_initial_state, void *workspace,
+                         size_t workspace_bytes, fbla_stream_t stream);
+/* One token per row: x (batch, channels) with x_stride[0], y contiguous; state (batch, width - 1,
+ * channels) is read and moved on by this token in place.  seq_len is not used.               */
+int fbla_causal_conv_step(const fbla_conv_problem *p, const void *x, const void *w, const void *bias,
+                          void *state, void *y, fbla_stream_t stream);
+
+/* ---- selective scan --------------------------------------------------------------------------
+ *   d = dt + dt_bias (softplus'd with softplus = 1; beyond 20 softplus is the identity)
+ *   h[c,n] <- exp(d A[c,n]) h[c,n] + d x[t,c] B[t,g,n]
+ *   y[t,c] = (sum_n C[t,g,n] h[c,n] + D[c] x[t,c]) * z sigmoid(z),   g = c / (channels / groups)
+ * x, dt, z, dy (batch, seq_len, channels) and B, C (batch, seq_len, groups, states) of `dtype`
+ * with the given strides (elements), the last dimension contiguous; y, dx, ddt, dz, dB, dC
+ * contiguous; A (channels, states), D, dt_bias (channels) and their gradients fp32.  States
+ * (sequences, channels, states) fp32, 16-byte aligned.  D, z, dt_bias, initial_state, final_state,
+ * d_final_state, d_initial_state, dD, d_dt_bias may be NULL.  checkpoints: fp32, 16-byte aligned,
+ * fbla_selective_scan_checkpoint_floats() of them; NULL when no backward follows.  Packed
+ * sequences: batch 1, cu_seqlens; tokens that no sequence owns come out as zeros, so do their
+ * gradients.  All arithmetic is fp32; no atomics.  No counterpart in the reference.           */
+typedef struct fbla_scan_problem {
+    int32_t dtype;
+    int32_t batch;          /* at most 65535                                            */
+    int32_t channels;
+    int32_t states;         /* 1..32                                                    */
+    int32_t groups;         /* divides channels                                         */
+    int32_t softplus;
+    int32_t num_seqs;       /* packed only, at most 65535                               */
+    int32_t reserved;
+    int64_t seq_len;
+    int64_t x_stride[2], dt_stride[2], z_stride[2], dy_stride[2];   /* batch, token     */
+    int64_t b_stride[3], c_stride[3];                               /* batch, token, group */
+    const int32_t *cu_seqlens;
+} fbla_scan_problem;
+
+int64_t fbla_selective_scan_checkpoint_floats(const fbla_scan_problem *p);
+/* Bytes of scratch of the forward (backward = 0) or the backward call; <0 on error. */
+int64_t fbla_selective_scan_workspace_bytes(const fbla_scan_problem *p, int backward);
+int fbla_selective_scan_fwd(const fbla_scan_problem *p, const void *x, const void *dt, const float *A,
+                            const void *B, const void *C, const float *D, const void *z,
+                            const float *dt_bias, const float *initial_state, void *y,
+                            float *final_state, float *checkpoints, void *workspace,
+                            size_t workspace_bytes, fbla_stream_t stream);
+int fbla_selective_scan_bwd(const fbla_scan_problem *p, const void *x, const void *dt, const float *A,
+                            const void *B, const void *C, const float *D, const void *z,
+                            const float *dt_bias, const float *initial_state, const float *checkpoints,
+                            const void *dy, const float *d_final_state, void *dx, void *ddt, float *dA,
+                            void *dB, void *dC, float *dD, void *dz, float *d_dt_bias,
+                            float *d_initial_state, void *workspace, size_t workspace_bytes,
+                            fbla_stream_t stream);
+/* One token per row: x, dt, z (batch, channels), B, C (batch, groups, states) with the batch (and
+ * group) strides; y contiguous; state (batch, channels, states) fp32 is moved on in place.
+ * seq_len is not used.                                                                       */
+int fbla_selective_scan_step(const fbla_scan_problem *p, const void *x, const void *dt, const float *A,
+                             const void *B, const void *C, const float *D, const void *z,
+                             const float *dt_bias, float *state, void *y, fbla_stream_t stream);
+
 /* The status word the kernels write when a bounded wait gives up (0 = none did; otherwise a number
  * naming the wait).  While it is non-zero every launching call returns FBLA_ERR_DEVICE.  Clear it
  * once the cause is dealt with; results of the failed call are invalid.  No counterpart in the

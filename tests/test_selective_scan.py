@@ -1,0 +1,284 @@
+"""Selective scan: formulas and refusals on the CPU, the kernels on the GPU.
+
+Tolerances, in fp32 roundings (2^-24) relative to the sum of the absolute terms.  A decay a = exp(d A) has
+the error of d (softplus: 4 units, weighted by |d A| a <= 0.37), of the product, and of the exponential
+(2^-22 at most): 6; with the rounding of h itself 7, and d x B three: a state that remembers L tokens is
+within 8 L + 8, and a gradient, which runs through the states and back, within twice that.  y adds N
+products and sums and the gate (the sigmoid is good to 2^-21: 8 units): N + 16.  dB, dC add one per channel
+summed, dA, dD and dbias one per token."""
+import pytest
+import torch
+
+from oracle import seq_oracle as Q
+from seq_helpers import DTYPES, cuda, leaf, randn, within
+
+from flash_bla.ops.selective_scan.naive import by_sequence, naive_selective_scan
+from flash_bla.ops.selective_scan.scan import selective_scan, selective_scan_step
+
+NAMES = ("x", "dt", "A", "B", "C", "D", "z", "bias", "init")
+GRADS = ("dx", "ddt", "dA", "dB", "dC", "dD", "dz", "dbias", "dinit")
+
+
+def inputs(seed, lead, C, G, N, dtype, rows, D=True, z=True, bias=True, state=True):
+    rn = randn(seed)
+    t = dict(x=rn(*lead, C, dtype=dtype), dt=rn(*lead, C, dtype=dtype, scale=0.5, shift=0.0 if bias else -3.0),
+             A=-torch.exp(rn(C, N, scale=0.8)), B=rn(*lead, G, N, dtype=dtype), C=rn(*lead, G, N, dtype=dtype),
+             D=rn(C) if D else None, z=rn(*lead, C, dtype=dtype) if z else None, bias=rn(C, shift=-3.0) if bias else None,
+             init=rn(rows, C, N) if state else None)
+    return t, rn(*lead, C, dtype=dtype), rn(rows, C, N)
+
+
+# ---- CPU ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cu", [None, [0, 1, 1, 4, 11]])
+@pytest.mark.parametrize("softplus", [False, True])
+def test_oracle_matches_autograd_and_differences(cu, softplus):
+    T, C, G, N = 11, 6, 2, 3
+    rows = 2 if cu is None else len(cu) - 1
+    t, dy, df = inputs(0, (2, T) if cu is None else (T,), C, G, N, torch.float64, rows)
+    t = {k: v.double().requires_grad_() for k, v in t.items()}
+    df = df.double()
+    order = ("x", "dt", "B", "C", "z")
+
+    def fwd(t):
+        if cu is None:
+            return naive_selective_scan(t["x"], t["dt"], t["A"], t["B"], t["C"], t["D"], t["z"], t["bias"], softplus, t["init"])
+        return by_sequence(lambda v, s: naive_selective_scan(v[0], v[1], t["A"], v[2], v[3], t["D"], v[4], t["bias"], softplus, s),
+                           torch.tensor(cu), [t[k] for k in order], t["init"])
+
+    y, f = fwd(t)
+    grads = torch.autograd.grad((y, f), [t[k] for k in NAMES], (dy, df))
+    lift = (lambda v: v) if cu is None else (lambda v: v[None])
+    ref = Q.scan(lift(t["x"]), lift(t["dt"]), t["A"], lift(t["B"]), lift(t["C"]), t["D"], lift(t["z"]), t["bias"], softplus, t["init"],
+                 lift(dy), df, None if cu is None else torch.tensor(cu))
+    assert torch.allclose(lift(y), ref["y"], atol=1e-11) and torch.allclose(f, ref["final"], atol=1e-11)
+    for got, name, key in zip(grads, NAMES, GRADS):
+        assert torch.allclose(lift(got) if name in order else got, ref[key], atol=1e-10), key
+    e = torch.zeros_like(t["A"])
+    e[1, 2] = 1e-6
+    num = sum(((p - m) * g).sum() for p, m, g in zip(fwd(dict(t, A=t["A"] + e)), fwd(dict(t, A=t["A"] - e)), (dy, df))) / 2e-6
+    # Rounding: both sums are within 100 roundings (8 per token and the sum's own) of 2^-53 of their absolute
+    # terms, whose difference is divided by 2e-6.  Truncation: the third derivative is at most (sum d)^2 < 40^2
+    # times the first, by 1e-12 / 6.  Without softplus a negative step size lets a state grow without bound, and
+    # the terms with it, so neither is an absolute number.
+    terms = sum((v.abs() * g.abs()).sum() for v, g in zip((y, f), (dy, df))).item()
+    assert abs(num.item() - ref["dA"][1, 2].item()) < 100 * 2.0 ** -53 * 2 * terms / 2e-6 + 1e-9 * abs(ref["dA"][1, 2].item())
+
+
+def test_refusals_on_cpu():
+    t, _, _ = inputs(1, (2, 5), 6, 2, 4, torch.float32, 2)
+
+    def refused(exc, match, step=False, **kw):
+        a = dict(t, **{k: v for k, v in kw.items() if k in t})
+        kw = {k: v for k, v in kw.items() if k not in t}
+        with pytest.raises(exc, match=match):
+            selective_scan(a["x"], a["dt"], a["A"], a["B"], a["C"], a["D"], a["z"], a["bias"], initial_state=a["init"], **kw)
+
+    refused(RuntimeError, "CUDA")
+    refused(ValueError, "shape", x=t["x"][0])
+    refused(TypeError, "dtype", x=t["x"].double())
+    refused(ValueError, "dt must", dt=t["dt"][:, :4])
+    refused(ValueError, "z must", z=t["z"].half())
+    refused(ValueError, "A must", A=t["A"].half())
+    refused(ValueError, "A must", A=t["A"][:5])
+    refused(ValueError, "states", A=torch.zeros(6, 33))
+    refused(ValueError, "B must", B=t["B"][..., :3])
+    refused(ValueError, "C must", C=t["C"].half())
+    refused(ValueError, "same shape", C=t["C"][:, :, :1])
+    refused(ValueError, "groups", B=torch.zeros(2, 5, 4, 4), C=torch.zeros(2, 5, 4, 4))
+    refused(ValueError, "groups", B=torch.zeros(2, 5, 0, 4), C=torch.zeros(2, 5, 0, 4))
+    refused(ValueError, "D must", D=t["D"].half())
+    refused(ValueError, "dt_bias must", bias=t["bias"][:5])
+    refused(ValueError, "initial_state", init=t["init"][:1])
+    refused(ValueError, "initial_state", init=t["init"].double())
+    refused(ValueError, "no channels", x=t["x"][..., :0])
+    refused(ValueError, "shape", cu_seqlens=torch.tensor([0, 5], dtype=torch.int32))
+
+    def step_refused(exc, match, **kw):
+        a = dict(x=t["x"][:, 0], dt=t["dt"][:, 0], A=t["A"], B=t["B"][:, 0], C=t["C"][:, 0], state=t["init"])
+        with pytest.raises(exc, match=match):
+            selective_scan_step(**dict(a, **kw))
+
+    step_refused(RuntimeError, "CUDA")
+    step_refused(ValueError, "shape", x=t["x"])
+    step_refused(ValueError, "state", state=t["init"][:1])
+    step_refused(ValueError, "contiguous", state=torch.zeros(2, 4, 6).transpose(1, 2))
+    step_refused(ValueError, "aligned", state=torch.zeros(2 * 6 * 4 + 1)[1:].view(2, 6, 4))
+    step_refused(RuntimeError, "gradient", A=t["A"].clone().requires_grad_())
+
+
+def test_library_refuses_without_a_device():
+    import ctypes
+    from flash_bla import _C
+    L = _C.lib()
+    ok = lambda: _C.ScanProblem(1, 2, 64, 16, 1, 1, 0, 0, 100)      # noqa: E731
+    p = ok()
+    assert L.fbla_selective_scan_checkpoint_floats(ctypes.byref(p)) > 0
+    assert L.fbla_selective_scan_workspace_bytes(ctypes.byref(p), 1) > 0
+    assert L.fbla_selective_scan_fwd(ctypes.byref(p), *[None] * 13, 0, None) == 1 and b"NULL" in L.fbla_last_error()
+    for field, value, word in (("states", 33, b"states"), ("states", 0, b"states"), ("groups", 3, b"groups"), ("dtype", 5, b"dtype"),
+                               ("channels", 0, b"channels"), ("seq_len", -1, b"seq_len"), ("batch", 70000, b"batch")):
+        bad = ok()
+        setattr(bad, field, value)
+        assert L.fbla_selective_scan_workspace_bytes(ctypes.byref(bad), 0) == -1 and word in L.fbla_last_error()
+    a = [16] * 10
+    assert L.fbla_selective_scan_step(ctypes.byref(p), *a[:8], 8, 16, None) == 1 and b"aligned" in L.fbla_last_error()
+
+
+# ---- GPU ------------------------------------------------------------------------------------------
+gpu = pytest.mark.gpu
+
+
+def run(t, dy, df, softplus, cu=None):
+    v = {k: leaf(x) for k, x in t.items()}
+    y, f = selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["bias"], dt_softplus=softplus,
+                          initial_state=v["init"], return_final_state=True, cu_seqlens=cuda(cu))
+    torch.autograd.backward((y, f), (dy.cuda(), df.cuda()))
+    return dict(y=y, final=f, **{g: None if v[k] is None else v[k].grad for k, g in zip(NAMES, GRADS)})
+
+
+def compare(got, t, dy, df, softplus, cu=None):
+    packed = cu is not None
+    lift = lambda v: v[None] if packed and v is not None else v     # noqa: E731
+    args = (lift(t["x"]), lift(t["dt"]), t["A"], lift(t["B"]), lift(t["C"]), t["D"], lift(t["z"]), t["bias"], softplus, t["init"],
+            lift(dy), df, cu)
+    ref, major = Q.scan(*args), Q.scan(*args, absolute=True)
+    T, (C, N) = lift(t["x"]).shape[1], t["A"].shape
+    tokens = t["x"].numel() // C
+    st = 8 * T + 8
+    k = dict(y=st + N + 16, final=st, dx=2 * st + N + 32, ddt=2 * st + N + 32, dA=2 * st + tokens + 32, dB=2 * st + C + 32,
+             dC=st + C + 32, dD=tokens + 32, dz=st + N + 32, dbias=2 * st + N + tokens + 32, dinit=2 * st + 32)
+    for key, n in k.items():
+        if got.get(key) is not None:
+            r, m = (d[key][0] if packed and key in ("y", "dx", "ddt", "dB", "dC", "dz") else d[key] for d in (ref, major))
+            within(got[key], r, m, n, key)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,C,G,N", [(1, 1, 1, 1, 1), (2, 3, 8, 1, 16), (2, 33, 70, 1, 16), (1, 64, 130, 2, 8), (3, 31, 64, 1, 5),
+                                       (1, 45, 24, 3, 32), (2, 19, 65, 1, 20), (1, 257, 16, 1, 3)])
+def test_forward_and_backward(dtype, B, T, C, G, N):
+    t, dy, df = inputs(T, (B, T), C, G, N, dtype, B)
+    compare(run(t, dy, df, True), t, dy, df, True)
+
+
+@gpu
+@pytest.mark.parametrize("missing", [("D",), ("z",), ("bias",), ("init",), ("D", "z", "bias", "init")])
+@pytest.mark.parametrize("softplus", [False, True])
+def test_optional_arguments(missing, softplus):
+    t, dy, df = inputs(5, (2, 40), 24, 1, 16, torch.bfloat16, 2, **{"state" if k == "init" else k: False for k in missing})
+    if not softplus:                    # step sizes are positive in earnest
+        t["dt"] = t["dt"].abs() * 0.2
+        t["bias"] = None if t["bias"] is None else t["bias"].abs() * 0.02
+    compare(run(t, dy, df, softplus), t, dy, df, softplus)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [1024, 1000])
+def test_segments(dtype, T):
+    """Few channels and many tokens: the tokens are cut into segments."""
+    t, dy, df = inputs(6, (1, T), 72, 1, 16, dtype, 1)
+    compare(run(t, dy, df, True), t, dy, df, True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [16, 8, 24])
+@pytest.mark.parametrize("cu", [[0, 1, 3, 6, 10, 47], [0, 0, 2, 2, 130, 131, 131], [0, 200], [2, 9, 40], [0, 300, 301, 700, 1000]])
+@pytest.mark.parametrize("state", [False, True])
+def test_packed(dtype, N, cu, state):
+    T = cu[-1] + 5                      # five tokens behind the last sequence
+    t, dy, df = inputs(T, (T,), 24, 1, N, dtype, len(cu) - 1, state=state)
+    t["B"][-3:] = float("nan")          # nothing of theirs may show anywhere
+    t["dt"][-2:] = float("inf")
+    cu = torch.tensor(cu, dtype=torch.int32)
+    got = run(t, dy, df, True, cu)
+    clean = dict(t, B=t["B"].nan_to_num(0.0), dt=t["dt"].nan_to_num(posinf=0.0))
+    compare(got, clean, dy, df, True, cu)
+    for key in ("y", "dx", "ddt", "dB", "dC", "dz"):
+        assert not got[key][:cu[0]].any() and not got[key][cu[-1]:].any(), key
+
+
+@gpu
+@pytest.mark.parametrize("off", [0, 1, 8])
+def test_strided_inputs_and_gradient(off):
+    """x and z as slices of one projection, B and C of another, at any offset; an expanded gradient."""
+    t, _, _ = inputs(8, (2, 50), 32, 1, 16, torch.bfloat16, 2, state=False)
+    xz = torch.cat((torch.zeros(2, 50, off, dtype=torch.bfloat16), t["x"], t["z"]), -1).cuda()
+    bc = torch.cat((torch.zeros(2, 50, 3, dtype=torch.bfloat16), t["B"].flatten(2), t["C"].flatten(2)), -1).cuda()
+    v = {k: leaf(x) for k, x in t.items()}
+    v["x"], v["z"] = (xz[..., off + i * 32:off + (i + 1) * 32].requires_grad_() for i in range(2))
+    v["B"], v["C"] = (bc[..., 3 + i * 16:19 + i * 16].requires_grad_() for i in range(2))      # no group dimension
+    g = randn(1)(2, 1, 32, dtype=torch.bfloat16)
+    y = selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["bias"], dt_softplus=True)
+    y.backward(g.cuda().expand(2, 50, 32))
+    got = dict(y=y, **{gr: v[k].grad for k, gr in zip(NAMES, GRADS) if v[k] is not None})
+    for k in ("dB", "dC"):
+        got[k] = got[k].unflatten(-1, (1, 16))
+    compare(got, t, g.expand(2, 50, 32), None, True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,C,G,N", [(1, 1, 1, 1), (3, 70, 1, 16), (2, 64, 2, 8), (2, 24, 1, 30)])
+def test_steps_continue_a_prompt(dtype, B, C, G, N):
+    T, n = 21, 4
+    t, _, _ = inputs(C, (B, T + n), C, G, N, dtype, B)
+    ref = Q.scan(t["x"], t["dt"], t["A"], t["B"], t["C"], t["D"], t["z"], t["bias"], True, t["init"])
+    major = Q.scan(t["x"], t["dt"], t["A"], t["B"], t["C"], t["D"], t["z"], t["bias"], True, t["init"], absolute=True)
+    k = 8 * (T + n) + 8
+    part = lambda lo, hi: {n_: cuda(v) if v is None or n_ in ("A", "D", "bias", "init") else v[:, lo:hi].cuda() for n_, v in t.items()}  # noqa: E731
+    v = part(0, T)
+    with torch.no_grad():
+        _, state = selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["bias"], dt_softplus=True,
+                                  initial_state=v["init"], return_final_state=True)
+        for i in range(T, T + n):
+            v = {n_: x if n_ in ("A", "D", "bias", "init") else x[:, 0] for n_, x in part(i, i + 1).items()}
+            y = selective_scan_step(v["x"], v["dt"], v["A"], v["B"], v["C"], state, v["D"], v["z"], v["bias"], dt_softplus=True)
+            within(y, ref["y"][:, i], major["y"][:, i], k + N + 16, f"token {i}")
+    within(state, ref["final"], major["final"], k, "state")
+
+
+@gpu
+def test_slow_decays_do_not_drift():
+    """A state that forgets almost nothing over 4096 tokens: the decays' errors must not add up one way.
+    Every factor is within one rounding of fp32 of its value (2^-24) and so is every step of the state, so
+    4096 steps are within 2 * 4096 roundings; a biased exponential (2^-22 each) would be four times that
+    and is seen here as a relative error of the state beyond 2^-24 * 4096."""
+    T = 4096
+    x = torch.zeros(1, T, 64)
+    x[0, 0] = 1.0
+    dt = torch.full((1, T, 64), 1.0)
+    A = -torch.logspace(-6, -3.5, 64)[:, None]
+    one = torch.ones(1, T, 1)
+    _, end = selective_scan(x.cuda(), dt.cuda(), A.cuda(), one.cuda(), one.cuda(), return_final_state=True)
+    ref = torch.exp(A.double() * (T - 1))
+    assert ((end[0].cpu().double() - ref).abs() <= 2.0 ** -24 * T * ref).all()
+
+
+@gpu
+def test_large_steps_and_masked_tokens():
+    """A step size far beyond 20 (softplus is the identity), one that underflows, infinities in x of one channel."""
+    t, dy, df = inputs(9, (1, 37), 16, 1, 16, torch.float32, 1)
+    t["dt"][0, 3] = 60.0
+    t["dt"][0, 4] = -200.0
+    compare(run(t, dy, df, True), t, dy, df, True)
+    t["x"][0, 5, 2] = float("inf")
+    y = selective_scan(*(cuda(t[k]) for k in NAMES[:8]), dt_softplus=True).cpu()
+    rest = torch.arange(16) != 2
+    assert y[0, :, rest].isfinite().all() and y[0, :5].isfinite().all() and not y[0, 5:, 2].isfinite().any()
+
+
+@gpu
+def test_same_bits_on_every_run_and_empty_inputs():
+    t, dy, df = inputs(10, (2, 515), 72, 1, 16, torch.float32, 2)
+    a, b = (run(t, dy, df, True) for _ in range(2))
+    assert all(torch.equal(a[k], b[k]) for k in a)
+    e = {k: (v if k in ("A", "D", "bias", "init") else v[:, :0]) for k, v in t.items()}
+    got = run(e, dy[:, :0], df, True)
+    assert got["y"].shape == (2, 0, 72) and torch.equal(got["final"], t["init"].cuda()) and torch.equal(got["dinit"], df.cuda())
+    assert not got["dA"].any() and not got["dD"].any() and not got["dbias"].any()
+    e = {k: (v if k in ("A", "D", "bias") else v[:0]) for k, v in t.items()}
+    got = run(e, dy[:0], df[:0], True)
+    assert got["y"].shape == (0, 515, 72) and not got["dA"].any()
