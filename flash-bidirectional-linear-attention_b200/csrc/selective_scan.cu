@@ -31,12 +31,15 @@ using fbla::from_f;
 using fbla::to_f;
 using fbla::seq::Pack;
 using fbla::seq::seq_of;
+using fbla::seq::F2;
+using fbla::seq::fma2;
+using fbla::seq::mul2;
 
 constexpr int kCB = 64;             // channels of a CTA
 constexpr int kThreads = 4 * kCB;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPad = kCB + 8;       // row of a per-token, per-channel float array: the four lanes of a channel write
-                                    // four rows at once, 8 banks apart
+constexpr int kPad = kCB + 8;       // row of a per-token, per-channel array: the four lanes of a channel write four rows
+                                    // at once, 8 banks apart
 
 struct ScanParams {
     int batch, channels, states, groups, softplus, num_seqs;
@@ -58,60 +61,90 @@ template <int NS> struct Tile {
     static constexpr int kTPR = kThreads / kTok;        // threads per token then
 };
 
-// 2^x for the decay of a state, x = d A log2(e).  |x| < 1/4: Taylor polynomial of degree 5 (next term
-// (x ln2)^6 / 6! < 4e-8), 1 exactly at 0, error of the order of one rounding: a state with such a decay
-// remembers many steps and a systematic error would add up over them.  Elsewhere the special function
-// unit's 2^-22 is good enough, as the state forgets it within a few steps.
-__device__ __forceinline__ float decay(float x) {
-    float p = 1.3333558e-3f;                // ln2^5 / 5!
-    p = fmaf(p, x, 9.6181291e-3f);          // ln2^4 / 4!
-    p = fmaf(p, x, 5.5504109e-2f);          // ln2^3 / 3!
-    p = fmaf(p, x, 0.24022651f);            // ln2^2 / 2!
-    p = fmaf(p, x, 0.69314718f);            // ln2
-    p = fmaf(p, x, 1.f);
-    return fabsf(x) < 0.25f ? p : exp2f(x);
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
-__device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(fbla::seq::exp_of(v)); }
+// 2^x for the decays of two states, x = d A log2(e).  |x| < 1/8: Taylor polynomial of degree 4 (next term
+// (x ln2)^5 / 5! < 4e-8), 1 exactly at 0, error of the order of one rounding.  Elsewhere the special function
+// unit: measured on B200 it is off by -2e-8 on average between -0.25 and 0, -5e-8 below, so over the 12 steps
+// that a state with x = -1/8 remembers, 2e-7 -- but over the thousands of steps of a slow state an error that
+// always has the same sign would be the largest of all.
+__device__ __forceinline__ F2 decay2(F2 x) {
+    F2 p(9.6181291e-3f);                            // ln2^4 / 4!
+    p = fma2(p, x, F2(5.5504109e-2f));              // ln2^3 / 3!
+    p = fma2(p, x, F2(0.24022651f));                // ln2^2 / 2!
+    p = fma2(p, x, F2(0.69314718f));
+    p = fma2(p, x, F2(1.f));
+    float x0, x1, p0, p1;
+    x.get(x0, x1);
+    p.get(p0, p1);
+    const float e0 = ex2(x0), e1 = ex2(x1);
+    return F2(fabsf(x0) < 0.125f ? p0 : e0, fabsf(x1) < 0.125f ? p1 : e1);
+}
 
-// NS consecutive floats at a 4*NS-byte boundary
-template <int NS> __device__ __forceinline__ void load_ns(const float* p, float (&v)[NS]) {
-    Pack<float, NS> k;
-    k.load(p);
+// A lane's NS states as pairs
+template <int NS> struct States {
+    F2 v[NS / 2];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) v[i] = k.e[i];
-}
-template <int NS> __device__ __forceinline__ void store_ns(float* p, const float (&v)[NS]) {
-    Pack<float, NS> k;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) k.e[i] = v[i];
-    k.store(p);
-}
-// Lane's states of a caller's (.., channels, N) tensor; the ones behind N are zero.
-template <int NS> __device__ __forceinline__ void load_user(const float* row, int n0, int N, float (&v)[NS]) {
-    if (N == 4 * NS) {
-        load_ns<NS>(row + n0, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) v[i] = n0 + i < N ? row[n0 + i] : 0.f;
+        for (int i = 0; i < NS / 2; ++i) v[i] = F2(0.f);
     }
-}
-template <int NS> __device__ __forceinline__ void store_user(float* row, int n0, int N, const float (&v)[NS]) {
-    if (N == 4 * NS) {
-        store_ns<NS>(row + n0, v);
-    } else {
+    __device__ __forceinline__ void load(const float* p) {      // aligned to 4 * NS bytes
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (n0 + i < N) row[n0 + i] = v[i];
+        for (int i = 0; i < NS / 4; ++i) {
+            const ulonglong2 w = reinterpret_cast<const ulonglong2*>(p)[i];
+            v[2 * i].v = w.x;
+            v[2 * i + 1].v = w.y;
+        }
+        if (NS == 2) v[0].v = *reinterpret_cast<const unsigned long long*>(p);
     }
-}
+    __device__ __forceinline__ void store(float* p) const {
+#pragma unroll
+        for (int i = 0; i < NS / 4; ++i) reinterpret_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i].v, v[2 * i + 1].v);
+        if (NS == 2) *reinterpret_cast<unsigned long long*>(p) = v[0].v;
+    }
+    // A caller's (.., channels, N) tensor; the states behind N are zero.
+    __device__ __forceinline__ void load_user(const float* row, int n0, int N) {
+        if (N == 4 * NS) {
+            load(row + n0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS / 2; ++i) {
+                const int n = n0 + 2 * i;
+                v[i] = F2(n < N ? row[n] : 0.f, n + 1 < N ? row[n + 1] : 0.f);
+            }
+        }
+    }
+    __device__ __forceinline__ void store_user(float* row, int n0, int N) const {
+        if (N == 4 * NS) {
+            store(row + n0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS / 2; ++i) {
+                const int n = n0 + 2 * i;
+                if (n < N) row[n] = v[i].x();
+                if (n + 1 < N) row[n + 1] = v[i].y();
+            }
+        }
+    }
+    __device__ __forceinline__ float sum() const {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS / 2; ++i) s += v[i].x() + v[i].y();
+        return s;
+    }
+};
 
 // Where this CTA and lane stand.
 template <int NS> struct Place {
     int64_t b;
     int seg, group, c0, cend;   // c0: first channel of the CTA, cend: end of its group
     int tile_in_group;
-    int warp, lane, q, cl, c;   // q: which states, cl / c: the lane's channel in the CTA / at all
+    int warp, lane, q;          // q: which states the lane holds
+    int pos, c;                 // the lane's channel: its position in a row of shared memory, its number
     bool live;
     __device__ __forceinline__ Place(const ScanParams& p) {
         const int cpg = p.channels / p.groups, tpg = (cpg + kCB - 1) / kCB;
@@ -124,10 +157,15 @@ template <int NS> struct Place {
         warp = threadIdx.x >> 5;
         lane = threadIdx.x & 31;
         q = lane & 3;
-        cl = warp * 8 + (lane >> 2);
-        c = c0 + cl;
+        pos = warp * 8 + (lane >> 2);
+        c = c0 + (pos % Tile<NS>::kTPR) * Tile<NS>::kVPT + pos / Tile<NS>::kTPR;
         live = c < cend;
     }
+    // When a tile is loaded or stored a thread has kVPT consecutive channels of one token, and the i-th of them
+    // lies at slot(i): threads next to each other write next to each other, and so read the lanes of a warp.
+    __device__ __forceinline__ static int row() { return threadIdx.x / Tile<NS>::kTPR; }
+    __device__ __forceinline__ static int col() { return threadIdx.x % Tile<NS>::kTPR * Tile<NS>::kVPT; }
+    __device__ __forceinline__ static int slot(int i) { return i * Tile<NS>::kTPR + threadIdx.x % Tile<NS>::kTPR; }
 };
 
 // Packed sequences: what happens at a token of the tile.
@@ -155,26 +193,27 @@ __device__ __forceinline__ void fill_marks(const ScanParams& p, Marks* m, int64_
 
 // The state that token `tt` of the tile continues from: that of the token before it, unless a sequence begins.
 template <int NS, bool VARLEN>
-__device__ __forceinline__ void state_before(const ScanParams& p, const Place<NS>& at, const Marks& m, int tt, const float* init,
-                                             const float (&h)[NS], float (&hp)[NS]) {
-    const int f = VARLEN ? m.first[tt] : -1;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) hp[i] = VARLEN && f >= 0 ? 0.f : h[i];
-    if (VARLEN && f >= 0 && init != nullptr && at.live)
-        load_user<NS>(init + ((int64_t)f * p.channels + at.c) * p.states, at.q * NS, p.states, hp);
+__device__ __forceinline__ States<NS> state_before(const ScanParams& p, const Place<NS>& at, const Marks& m, int tt, const float* init,
+                                                   const States<NS>& h) {
+    States<NS> r = h;
+    if (VARLEN) {
+        const int f = m.first[tt];
+        if (f >= 0) {
+            r.zero();
+            if (init != nullptr && at.live) r.load_user(init + ((int64_t)f * p.channels + at.c) * p.states, at.q * NS, p.states);
+        }
+    }
+    return r;
 }
 
 // V elements of one token's row from channel c, zeros behind cend.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* row, int c, int cend, bool vec, float (&out)[V]) {
+__device__ __forceinline__ void load_row(const T* row, int c, int cend, bool vec, Pack<T, V>& out) {
     if (vec && c + V <= cend) {
-        Pack<T, V> k;
-        k.load(row + c);
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = k.get(i);
+        out.load(row + c);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = c + i < cend ? to_f<T>(row[c + i]) : 0.f;
+        for (int i = 0; i < V; ++i) out.e[i] = c + i < cend ? row[c + i] : from_f<T>(0.f);
     }
 }
 template <typename T, int V>
@@ -191,20 +230,29 @@ __device__ __forceinline__ void store_row(T* row, int c, int cend, bool vec, con
     }
 }
 
-// One of B, C for the tokens [t0, t0 + kTok) into dst[token][kNP]; zeros behind N, behind `end`, and for
-// tokens of no sequence.
-template <typename T, int NS, bool VARLEN>
-__device__ __forceinline__ void stage_bc(const T* src, const int64_t (&st)[3], const ScanParams& p, const Place<NS>& at, int64_t t0,
-                                         int64_t end, const Marks* m, float* dst) {
+// A thread's share of B (or C) of a tile: loaded while the tile before is worked on, then put in place.  Zeros
+// behind N, behind `end`, and for tokens of no sequence.
+template <typename T, int NS> struct BCShare {
     using L = Tile<NS>;
-    const T* base = src + at.b * st[0] + at.group * st[2];
-    for (int i = threadIdx.x; i < L::kTok * L::kNP; i += kThreads) {
-        const int t = i / L::kNP, n = i % L::kNP;
-        bool ok = n < p.states && t0 + t < end;
-        if (VARLEN) ok = ok && m->inside[t];
-        dst[i] = ok ? to_f<T>(base[(t0 + t) * st[1] + n]) : 0.f;
+    static constexpr int kEach = L::kTok * L::kNP / kThreads;
+    T v[kEach];
+    __device__ __forceinline__ void load(const T* src, const int64_t (&st)[3], const ScanParams& p, const Place<NS>& at, int64_t t0,
+                                         int64_t end) {
+        const T* base = src + at.b * st[0] + at.group * st[2];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int i = threadIdx.x + k * kThreads, t = i / L::kNP, n = i % L::kNP;
+            v[k] = n < p.states && t0 + t < end ? base[(t0 + t) * st[1] + n] : from_f<T>(0.f);
+        }
     }
-}
+    template <bool VARLEN> __device__ __forceinline__ void put(float* dst, const Marks& m) const {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int i = threadIdx.x + k * kThreads;
+            dst[i] = !VARLEN || m.inside[i / L::kNP] ? to_f<T>(v[k]) : 0.f;
+        }
+    }
+};
 
 // Lane q of the four gets the sum over them of v[q].
 __device__ __forceinline__ float sum4(const float (&v)[4], int q) {
@@ -220,50 +268,77 @@ template <int NS> __device__ __forceinline__ int64_t seg_at(const ScanParams& p,
     return (b * p.segs + seg) * p.channels + c;
 }
 
-template <typename T, int NS> struct FwdSmem {
+template <int NS> struct FwdSmem {
     using L = Tile<NS>;
-    float2 dx[L::kTok][kCB];            // (d, d x)
+    float2 dx[L::kTok][kPad];           // (d, d x)
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
     float y[L::kTok][kPad];
+    float D[kCB], bias[kCB];            // by slot
     Marks marks;
 };
 
 // LOCAL: end state of the segment from zero, and the sum of d (infinite when a sequence begins inside, so
-// that nothing from before gets through).  Otherwise the outputs.
+// that nothing from before gets through).  Otherwise the outputs.  What the next tile needs from global memory
+// is on its way while a tile is worked on.
 template <typename T, int NS, bool VARLEN, bool LOCAL>
-__global__ void __launch_bounds__(kThreads) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
-                                                            const T* __restrict__ Bm, const T* __restrict__ Cm,
-                                                            const T* __restrict__ z, const float* __restrict__ init,
-                                                            T* __restrict__ y, float* __restrict__ fin, float* __restrict__ ckpt,
-                                                            float* __restrict__ seg_h, float* __restrict__ seg_d) {
+__global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
+                                                               const T* __restrict__ Bm, const T* __restrict__ Cm,
+                                                               const T* __restrict__ z, const float* __restrict__ init,
+                                                               T* __restrict__ y, float* __restrict__ fin, float* __restrict__ ckpt,
+                                                               float* __restrict__ seg_h, float* __restrict__ seg_d) {
     using L = Tile<NS>;
+    constexpr int V = L::kVPT;
     extern __shared__ __align__(16) unsigned char raw_smem[];
-    FwdSmem<T, NS>& sm = *reinterpret_cast<FwdSmem<T, NS>*>(raw_smem);
+    FwdSmem<NS>& sm = *reinterpret_cast<FwdSmem<NS>*>(raw_smem);
     const Place<NS> at(p);
     if (LOCAL && at.seg == p.segs - 1) return;      // nothing comes behind it
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
 
-    float A2[NS], h[NS], sum_d = 0.f;
+    States<NS> A2, h;
+    float sum_d = 0.f;
+    A2.zero();
+    h.zero();
+    if (at.live) {
+        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        A2[i] = at.live && n0 + i < N ? p.A[(int64_t)at.c * N + n0 + i] * 1.44269504f : 0.f;
-        h[i] = 0.f;
-    }
-    if (!LOCAL && at.live) {
-        if (!VARLEN && init != nullptr) load_user<NS>(init + (at.b * p.channels + at.c) * N, n0, N, h);
-        for (int j = 0; j < at.seg; ++j) {
-            const int64_t k = seg_at<NS>(p, at.b, j, at.c);
-            const float sd = seg_d[k];
-            float own[NS];
-            load_ns<NS>(seg_h + k * L::kNP + n0, own);
+        for (int i = 0; i < NS / 2; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
+        if (!LOCAL) {
+            if (!VARLEN && init != nullptr) h.load_user(init + (at.b * p.channels + at.c) * N, n0, N);
+            for (int j = 0; j < at.seg; ++j) {
+                const int64_t k = seg_at<NS>(p, at.b, j, at.c);
+                const float sd = seg_d[k];
+                States<NS> own;
+                own.load(seg_h + k * L::kNP + n0);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = sd == INFINITY ? own[i] : fmaf(decay(sd * A2[i]), h[i], own[i]);
+                for (int i = 0; i < NS / 2; ++i)
+                    h.v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2.v[i])), h.v[i], own.v[i]);
+            }
         }
     }
-    const int row = threadIdx.x / L::kTPR, col = (threadIdx.x % L::kTPR) * L::kVPT;     // when loading or storing
+    const int row = at.row(), c = at.c0 + at.col();     // when loading or storing
+    if (row == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            sm.D[at.slot(i)] = p.D != nullptr && c + i < at.cend ? p.D[c + i] : 0.f;
+            sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
+        }
+    }
     const int64_t ntiles = (p.len + L::kTok - 1) / L::kTok;
 
+    Pack<T, V> px, pd;
+    BCShare<T, NS> pB, pC;
+    auto fetch = [&](int64_t tb) {
+        const int64_t t = tb + row;
+        if (t < t1) {
+            load_row<T, V>(x + at.b * p.xs[0] + t * p.xs[1], c, at.cend, p.vec, px);
+            load_row<T, V>(dt + at.b * p.ds[0] + t * p.ds[1], c, at.cend, p.vec, pd);
+        }
+        pB.load(Bm, p.bs, p, at, tb, t1);
+        if (!LOCAL) pC.load(Cm, p.cs, p, at, tb, t1);
+    };
+    fetch(t0);
+    __syncthreads();
     for (int64_t tb = t0; tb < t1; tb += L::kTok) {
         if (VARLEN) {
             fill_marks(p, &sm.marks, tb, L::kTok, t1);
@@ -272,74 +347,77 @@ __global__ void __launch_bounds__(kThreads) scan_fwd_kernel(const ScanParams p, 
         const int64_t t = tb + row;
         bool ok = t < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
-        float xv[L::kVPT], dv[L::kVPT];
-        if (ok) {
-            load_row<T, L::kVPT>(x + at.b * p.xs[0] + t * p.xs[1], at.c0 + col, at.cend, p.vec, xv);
-            load_row<T, L::kVPT>(dt + at.b * p.ds[0] + t * p.ds[1], at.c0 + col, at.cend, p.vec, dv);
+        Pack<T, V> cx, cz;
+        cx.zero();
+        if (ok) cx = px;
 #pragma unroll
-            for (int i = 0; i < L::kVPT; ++i) {
-                if (p.bias != nullptr && at.c0 + col + i < at.cend) dv[i] += p.bias[at.c0 + col + i];
-                if (p.softplus) dv[i] = softplus(dv[i]);
+        for (int i = 0; i < V; ++i) {
+            const int s = at.slot(i);
+            float d = 0.f;
+            if (ok) {
+                d = pd.get(i) + sm.bias[s];
+                if (p.softplus) d = fbla::seq::softplus(d);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < L::kVPT; ++i) xv[i] = dv[i] = 0.f;
+            sm.dx[row][s] = make_float2(d, d * cx.get(i));
         }
-#pragma unroll
-        for (int i = 0; i < L::kVPT; ++i) sm.dx[row][col + i] = make_float2(dv[i], dv[i] * xv[i]);
-        stage_bc<T, NS, VARLEN>(Bm, p.bs, p, at, tb, t1, &sm.marks, sm.B);
-        if (!LOCAL) stage_bc<T, NS, VARLEN>(Cm, p.cs, p, at, tb, t1, &sm.marks, sm.C);
+        pB.template put<VARLEN>(sm.B, sm.marks);
+        if (!LOCAL) pC.template put<VARLEN>(sm.C, sm.marks);
         __syncthreads();
 
-        if (!LOCAL && ckpt != nullptr && at.live)
-            store_ns<NS>(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0), h);
+        if (tb + L::kTok < t1) fetch(tb + L::kTok);
+        if (!LOCAL) {
+            if (z != nullptr && t < t1) load_row<T, V>(z + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, cz);
+            if (ckpt != nullptr && at.live) h.store(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0));
+        }
 #pragma unroll 2
         for (int tt = 0; tt < L::kTok; tt += 4) {
             float ys[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 v = sm.dx[tt + k][at.cl];
-                float Bv[NS], Cv[NS];
-                load_ns<NS>(sm.B + (tt + k) * L::kNP + n0, Bv);
-                if (!LOCAL) load_ns<NS>(sm.C + (tt + k) * L::kNP + n0, Cv);
-                float hp[NS];
-                state_before<NS, VARLEN>(p, at, sm.marks, tt + k, init, h, hp);
+                const float2 v = sm.dx[tt + k][at.pos];
+                const F2 d2(v.x), dx2(v.y);
+                States<NS> Bv, Cv;
+                Bv.load(sm.B + (tt + k) * L::kNP + n0);
+                if (!LOCAL) Cv.load(sm.C + (tt + k) * L::kNP + n0);
+                h = state_before<NS, VARLEN>(p, at, sm.marks, tt + k, init, h);
                 if (LOCAL) sum_d += VARLEN && sm.marks.first[tt + k] >= 0 ? INFINITY : v.x;
-                float acc = 0.f;
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    h[i] = fmaf(decay(v.x * A2[i]), hp[i], v.y * Bv[i]);
-                    if (!LOCAL) acc = fmaf(Cv[i], h[i], acc);
+                for (int i = 0; i < NS / 2; ++i) {
+                    h.v[i] = fma2(decay2(mul2(d2, A2.v[i])), h.v[i], mul2(dx2, Bv.v[i]));
                 }
-                ys[k] = acc;
+                if (!LOCAL) {
+                    F2 s2 = mul2(Cv.v[0], h.v[0]);
+#pragma unroll
+                    for (int i = 1; i < NS / 2; ++i) s2 = fma2(Cv.v[i], h.v[i], s2);
+                    ys[k] = s2.x() + s2.y();
+                }
                 if (VARLEN && !LOCAL && fin != nullptr) {
                     const int l = sm.marks.last[tt + k];
-                    if (l >= 0 && at.live) store_user<NS>(fin + ((int64_t)l * p.channels + at.c) * N, n0, N, h);
+                    if (l >= 0 && at.live) h.store_user(fin + ((int64_t)l * p.channels + at.c) * N, n0, N);
                 }
             }
-            if (!LOCAL) sm.y[tt + at.q][at.cl] = sum4(ys, at.q);
+            if (!LOCAL) sm.y[tt + at.q][at.pos] = sum4(ys, at.q);
         }
         __syncthreads();
         if (!LOCAL && t < t1) {
-            float out[L::kVPT], zv[L::kVPT];
-            if (z != nullptr) load_row<T, L::kVPT>(z + at.b * p.zs[0] + t * p.zs[1], at.c0 + col, at.cend, p.vec, zv);
+            float out[V];
 #pragma unroll
-            for (int i = 0; i < L::kVPT; ++i) {
-                float s = sm.y[row][col + i];
-                if (p.D != nullptr && at.c0 + col + i < at.cend) s = fmaf(p.D[at.c0 + col + i], xv[i], s);
-                if (z != nullptr) s *= zv[i] * fbla::seq::sigmoid<T>(zv[i]);
-                out[i] = ok ? s : 0.f;
+            for (int i = 0; i < V; ++i) {
+                const int s = at.slot(i);
+                float v = fmaf(sm.D[s], cx.get(i), sm.y[row][s]);
+                if (z != nullptr) v *= cz.get(i) * fbla::seq::sigmoid<T>(cz.get(i));
+                out[i] = ok ? v : 0.f;
             }
-            store_row<T, L::kVPT>(y + (at.b * p.len + t) * p.channels, at.c0 + col, at.cend, p.vec, out);
+            store_row<T, V>(y + (at.b * p.len + t) * p.channels, c, at.cend, p.vec, out);
         }
     }
     if (!at.live) return;
     if (LOCAL) {
         const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c);
-        store_ns<NS>(seg_h + k * L::kNP + n0, h);
+        h.store(seg_h + k * L::kNP + n0);
         if (at.q == 0) seg_d[k] = sum_d;
     } else if (!VARLEN && fin != nullptr && at.seg == p.segs - 1) {
-        store_user<NS>(fin + (at.b * p.channels + at.c) * N, n0, N, h);
+        h.store_user(fin + (at.b * p.channels + at.c) * N, n0, N);
     }
 }
 
@@ -353,110 +431,110 @@ __global__ void __launch_bounds__(256) scan_empty_kernel(const ScanParams p, con
     if (tokens <= 0) to[s * n + i] = from != nullptr ? from[s * n + i] : 0.f;
 }
 
-template <typename T, int NS> struct BwdSmem {
-    using L = Tile<NS>;
-    float4 v[L::kTok][kCB];                         // (d, d x, e, -)
-    float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
-    float start[L::kTok / L::kSub][kThreads][NS];   // each thread's states at the starts of the sub-tiles
-    float gB[L::kTok][kPad], rA[L::kTok][kPad], y[L::kTok][kPad];
-    float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its eight channels
-    float dD[kThreads][L::kVPT], db[kThreads][L::kVPT];
-    Marks marks;
-};
-
-// What a thread loads of a tile in the backward passes: d and the slope of d, x, e, and what dz needs.
-template <typename T, int V> struct BwdRow {
-    float x[V], d[V], slope[V], e[V], dy[V], zv[V];
-};
-
-template <typename T, int NS>
-__device__ __forceinline__ void load_bwd_row(const ScanParams& p, const Place<NS>& at, const T* x, const T* dt, const T* z, const T* dy,
-                                             int64_t t, int col, bool ok, BwdRow<T, Tile<NS>::kVPT>& r) {
-    constexpr int V = Tile<NS>::kVPT;
-    const int c = at.c0 + col;
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.x[i] = r.d[i] = r.slope[i] = r.e[i] = r.dy[i] = r.zv[i] = 0.f;
-    if (!ok) return;
-    if (x != nullptr) load_row<T, V>(x + at.b * p.xs[0] + t * p.xs[1], c, at.cend, p.vec, r.x);
-    load_row<T, V>(dt + at.b * p.ds[0] + t * p.ds[1], c, at.cend, p.vec, r.d);
-    load_row<T, V>(dy + at.b * p.gs[0] + t * p.gs[1], c, at.cend, p.vec, r.dy);
-    if (z != nullptr) load_row<T, V>(z + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, r.zv);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if (p.bias != nullptr && c + i < at.cend) r.d[i] += p.bias[c + i];
-        r.slope[i] = 1.f;
-        if (p.softplus) {
-            r.slope[i] = r.d[i] > 20.f ? 1.f : fbla::seq::sigmoid<float>(r.d[i]);
-            r.d[i] = softplus(r.d[i]);
-        }
-        r.e[i] = z != nullptr ? r.dy[i] * r.zv[i] * fbla::seq::sigmoid<float>(r.zv[i]) : r.dy[i];
+// What a thread loads of a tile in the backward passes, as it stands in memory.
+template <typename T, int NS> struct BwdShare {
+    static constexpr int V = Tile<NS>::kVPT;
+    Pack<T, V> x, dt, z, dy;
+    __device__ __forceinline__ void load(const ScanParams& p, const Place<NS>& at, const T* xp, const T* dtp, const T* zp, const T* dyp,
+                                         int64_t t) {
+        const int c = at.c0 + at.col();
+        if (xp != nullptr) load_row<T, V>(xp + at.b * p.xs[0] + t * p.xs[1], c, at.cend, p.vec, x);
+        load_row<T, V>(dtp + at.b * p.ds[0] + t * p.ds[1], c, at.cend, p.vec, dt);
+        load_row<T, V>(dyp + at.b * p.gs[0] + t * p.gs[1], c, at.cend, p.vec, dy);
+        if (zp != nullptr) load_row<T, V>(zp + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, z);
     }
-}
+    __device__ __forceinline__ float step(int i, float bias, int soft) const {
+        const float d = dt.get(i) + bias;
+        return soft ? fbla::seq::softplus(d) : d;
+    }
+    __device__ __forceinline__ float e(int i, bool gated) const {
+        const float g = dy.get(i);
+        return gated ? g * z.get(i) * fbla::seq::sigmoid<float>(z.get(i)) : g;
+    }
+};
 
-template <typename T, int NS> struct BwdLocalSmem {
+template <int NS> struct BwdLocalSmem {
     using L = Tile<NS>;
-    float2 v[L::kTok][kCB];             // (d, e)
+    float2 v[L::kTok][kPad];            // (d, e)
     float C[L::kTok * L::kNP];
+    float bias[kCB];
     Marks marks;
 };
 
 // What a segment passes to the one before it, from zero: a G of its first token.  seg_d as in the forward.
 template <typename T, int NS, bool VARLEN>
-__global__ void __launch_bounds__(kThreads) scan_bwd_local_kernel(const ScanParams p, const T* __restrict__ dt, const T* __restrict__ Cm,
-                                                                  const T* __restrict__ z, const T* __restrict__ dy,
-                                                                  const float* __restrict__ dfin, float* __restrict__ seg_g,
-                                                                  float* __restrict__ seg_d) {
+__global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanParams p, const T* __restrict__ dt, const T* __restrict__ Cm,
+                                                                     const T* __restrict__ z, const T* __restrict__ dy,
+                                                                     const float* __restrict__ dfin, float* __restrict__ seg_g,
+                                                                     float* __restrict__ seg_d) {
     using L = Tile<NS>;
     extern __shared__ __align__(16) unsigned char raw_smem[];
-    BwdLocalSmem<T, NS>& sm = *reinterpret_cast<BwdLocalSmem<T, NS>*>(raw_smem);
+    BwdLocalSmem<NS>& sm = *reinterpret_cast<BwdLocalSmem<NS>*>(raw_smem);
     const Place<NS> at(p);
     if (at.seg == 0) return;            // nothing comes before it
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
-    float A2[NS], g[NS], sum_d = 0.f;
+    States<NS> A2, g;
+    float sum_d = 0.f;
+    A2.zero();
+    g.zero();
+    if (at.live) {
+        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        A2[i] = at.live && n0 + i < N ? p.A[(int64_t)at.c * N + n0 + i] * 1.44269504f : 0.f;
-        g[i] = 0.f;
+        for (int i = 0; i < NS / 2; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
+        if (!VARLEN && dfin != nullptr && at.seg == p.segs - 1) g.load_user(dfin + (at.b * p.channels + at.c) * N, n0, N);
     }
-    if (!VARLEN && dfin != nullptr && at.live && at.seg == p.segs - 1) load_user<NS>(dfin + (at.b * p.channels + at.c) * N, n0, N, g);
-    const int row = threadIdx.x / L::kTPR, col = (threadIdx.x % L::kTPR) * L::kVPT;
-    for (int64_t tb = t0 + (t1 - 1 - t0) / L::kTok * L::kTok; tb >= t0; tb -= L::kTok) {
+    const int row = at.row(), c = at.c0 + at.col();
+    if (row == 0) {
+#pragma unroll
+        for (int i = 0; i < L::kVPT; ++i) sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
+    }
+    BwdShare<T, NS> next;
+    BCShare<T, NS> pC;
+    auto fetch = [&](int64_t tb) {
+        if (tb + row < t1) next.load(p, at, nullptr, dt, z, dy, tb + row);
+        pC.load(Cm, p.cs, p, at, tb, t1);
+    };
+    const int64_t tlast = t0 + (t1 - 1 - t0) / L::kTok * L::kTok;
+    fetch(tlast);
+    for (int64_t tb = tlast; tb >= t0; tb -= L::kTok) {
         __syncthreads();
         if (VARLEN) {
             fill_marks(p, &sm.marks, tb, L::kTok, t1);
             __syncthreads();
         }
-        const int64_t t = tb + row;
-        bool ok = t < t1;
+        bool ok = tb + row < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
-        BwdRow<T, L::kVPT> r;
-        load_bwd_row<T, NS>(p, at, nullptr, dt, z, dy, t, col, ok, r);
 #pragma unroll
-        for (int i = 0; i < L::kVPT; ++i) sm.v[row][col + i] = make_float2(r.d[i], r.e[i]);
-        stage_bc<T, NS, VARLEN>(Cm, p.cs, p, at, tb, t1, &sm.marks, sm.C);
+        for (int i = 0; i < L::kVPT; ++i) {
+            const int s = at.slot(i);
+            sm.v[row][s] = ok ? make_float2(next.step(i, sm.bias[s], p.softplus), next.e(i, z != nullptr)) : make_float2(0.f, 0.f);
+        }
+        pC.template put<VARLEN>(sm.C, sm.marks);
         __syncthreads();
+        if (tb > t0) fetch(tb - L::kTok);
+#pragma unroll 4
         for (int tt = L::kTok - 1; tt >= 0; --tt) {
-            const float2 v = sm.v[tt][at.cl];
-            float Cv[NS];
-            load_ns<NS>(sm.C + tt * L::kNP + n0, Cv);
+            const float2 v = sm.v[tt][at.pos];
+            const F2 d2(v.x), e2(v.y);
+            States<NS> Cv;
+            Cv.load(sm.C + tt * L::kNP + n0);
             if (VARLEN && dfin != nullptr) {
                 const int l = sm.marks.last[tt];
-                if (l >= 0 && at.live) load_user<NS>(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N, g);
+                if (l >= 0 && at.live) g.load_user(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N);
             }
             sum_d += v.x;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) g[i] = decay(v.x * A2[i]) * fmaf(v.y, Cv[i], g[i]);
+            for (int i = 0; i < NS / 2; ++i) g.v[i] = mul2(decay2(mul2(d2, A2.v[i])), fma2(e2, Cv.v[i], g.v[i]));
             if (VARLEN && sm.marks.first[tt] >= 0) {
                 sum_d = INFINITY;
-#pragma unroll
-                for (int i = 0; i < NS; ++i) g[i] = 0.f;
+                g.zero();
             }
         }
     }
     if (!at.live) return;
     const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c);
-    store_ns<NS>(seg_g + k * L::kNP + n0, g);
+    g.store(seg_g + k * L::kNP + n0);
     if (at.q == 0) seg_d[k] = sum_d;
 }
 
@@ -485,8 +563,24 @@ template <int M> __device__ __forceinline__ int sum8(float (&v)[M], int lane) {
     return first;
 }
 
-// All gradients of one segment.  part_bc: [channel tile of the group][batch][token][group][2][kNP] sums over the
-// CTA's channels; part_A [batch][segs][channels][N], part_D / part_bias [batch][segs][channels].
+template <int NS> struct BwdSmem {
+    using L = Tile<NS>;
+    static constexpr int kSubs = L::kTok / L::kSub;
+    float2 dx[L::kTok][kPad];                       // (d, d x); behind the reverse pass of a sub-tile (sum G B, sum A r)
+    float e[L::kTok][kPad];                         // e; then s = sum C h
+    float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
+    float start[kSubs][kThreads][NS];               // each thread's states at the starts of the sub-tiles
+    float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its eight channels
+    float dD[L::kVPT][kThreads], db[L::kVPT][kThreads];
+    float D[kCB], bias[kCB];
+    Marks marks;
+};
+
+// All gradients of one segment, tile after tile from its end.  In a tile the states are formed again from the
+// checkpoint, first up to the starts of its sub-tiles; then sub-tile after sub-tile, from the last one, with
+// the decays and states of its tokens in registers, the reverse recurrence.
+// part_bc: [channel tile of the group][batch][token][group][2][kNP] sums over the CTA's channels;
+// part_A [batch][segs][channels][N], part_D / part_bias [batch][segs][channels].
 template <typename T, int NS, bool VARLEN>
 __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt, const T* __restrict__ Bm, const T* __restrict__ Cm,
@@ -495,34 +589,43 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     T* __restrict__ ddt, T* __restrict__ dz, float* __restrict__ dinit, float* __restrict__ part_bc, float* __restrict__ part_A,
     float* __restrict__ part_D, float* __restrict__ part_bias) {
     using L = Tile<NS>;
-    constexpr int K = L::kSub;
+    constexpr int K = L::kSub, V = L::kVPT, P = NS / 2;
     extern __shared__ __align__(16) unsigned char raw_smem[];
-    BwdSmem<T, NS>& sm = *reinterpret_cast<BwdSmem<T, NS>*>(raw_smem);
+    BwdSmem<NS>& sm = *reinterpret_cast<BwdSmem<NS>*>(raw_smem);
     const Place<NS> at(p);
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
     const int64_t ntiles = (p.len + L::kTok - 1) / L::kTok;
 
-    float A[NS], g[NS], dA[NS];         // g: a G of the token behind
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        A[i] = at.live && n0 + i < N ? p.A[(int64_t)at.c * N + n0 + i] : 0.f;
-        g[i] = dA[i] = 0.f;
-    }
+    // A2 = A log2(e); sums with A itself are formed with A2 and scaled back once
+    States<NS> A2, g, dA;               // g: a G of the token behind
+    A2.zero();
+    g.zero();
+    dA.zero();
     if (at.live) {
-        if (!VARLEN && dfin != nullptr && at.seg == p.segs - 1) load_user<NS>(dfin + (at.b * p.channels + at.c) * N, n0, N, g);
+        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
+#pragma unroll
+        for (int i = 0; i < P; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
+        if (!VARLEN && dfin != nullptr && at.seg == p.segs - 1) g.load_user(dfin + (at.b * p.channels + at.c) * N, n0, N);
         for (int j = p.segs - 1; j > at.seg; --j) {
             const int64_t k = seg_at<NS>(p, at.b, j, at.c);
             const float sd = seg_d[k];
-            float own[NS];
-            load_ns<NS>(seg_g + k * L::kNP + n0, own);
+            States<NS> own;
+            own.load(seg_g + k * L::kNP + n0);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) g[i] = sd == INFINITY ? own[i] : fmaf(decay(sd * A[i] * 1.44269504f), g[i], own[i]);
+            for (int i = 0; i < P; ++i) g.v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2.v[i])), g.v[i], own.v[i]);
         }
     }
-    const int row = threadIdx.x / L::kTPR, col = (threadIdx.x % L::kTPR) * L::kVPT;
+    const int row = at.row(), c = at.c0 + at.col();
+    if (row == 0) {
 #pragma unroll
-    for (int i = 0; i < L::kVPT; ++i) sm.dD[threadIdx.x][i] = sm.db[threadIdx.x][i] = 0.f;
+        for (int i = 0; i < V; ++i) {
+            sm.D[at.slot(i)] = p.D != nullptr && c + i < at.cend ? p.D[c + i] : 0.f;
+            sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sm.dD[i][threadIdx.x] = sm.db[i][threadIdx.x] = 0.f;
 
     for (int64_t tb = t0 + (t1 - 1 - t0) / L::kTok * L::kTok; tb >= t0; tb -= L::kTok) {
         __syncthreads();
@@ -533,91 +636,99 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         const int64_t t = tb + row;
         bool ok = t < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
+        States<NS> h;
+        h.zero();
+        if (at.live) h.load(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0));
         {
-            BwdRow<T, L::kVPT> r;
-            load_bwd_row<T, NS>(p, at, x, dt, z, dy, t, col, ok, r);
+            BwdShare<T, NS> in;
+            if (ok) in.load(p, at, x, dt, z, dy, t);
+            BCShare<T, NS> bc;
+            bc.load(Bm, p.bs, p, at, tb, t1);
+            bc.template put<VARLEN>(sm.B, sm.marks);
+            bc.load(Cm, p.cs, p, at, tb, t1);
+            bc.template put<VARLEN>(sm.C, sm.marks);
 #pragma unroll
-            for (int i = 0; i < L::kVPT; ++i) sm.v[row][col + i] = make_float4(r.d[i], r.d[i] * r.x[i], r.e[i], 0.f);
+            for (int i = 0; i < V; ++i) {
+                const int s = at.slot(i);
+                const float d = ok ? in.step(i, sm.bias[s], p.softplus) : 0.f;
+                sm.dx[row][s] = make_float2(d, ok ? d * in.x.get(i) : 0.f);
+                sm.e[row][s] = ok ? in.e(i, z != nullptr) : 0.f;
+            }
         }
-        stage_bc<T, NS, VARLEN>(Bm, p.bs, p, at, tb, t1, &sm.marks, sm.B);
-        stage_bc<T, NS, VARLEN>(Cm, p.cs, p, at, tb, t1, &sm.marks, sm.C);
         __syncthreads();
 
-        // forward again: the states at the starts of the sub-tiles
-        float h[NS];
-#pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = 0.f;
-        if (at.live) load_ns<NS>(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0), h);
 #pragma unroll 1
-        for (int sub = 0; sub < L::kTok / K; ++sub) {
-            store_ns<NS>(sm.start[sub][threadIdx.x], h);
-            if (sub == L::kTok / K - 1) break;
+        for (int sub = 0; sub < BwdSmem<NS>::kSubs; ++sub) {
+            h.store(sm.start[sub][threadIdx.x]);
+            if (sub == BwdSmem<NS>::kSubs - 1) break;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
-                const float2 v = *reinterpret_cast<const float2*>(&sm.v[tt][at.cl]);
-                float Bv[NS];
-                load_ns<NS>(sm.B + tt * L::kNP + n0, Bv);
-                float hp[NS];
-                state_before<NS, VARLEN>(p, at, sm.marks, tt, init, h, hp);
+                const float2 v = sm.dx[tt][at.pos];
+                const F2 d2(v.x), dx2(v.y);
+                States<NS> Bv;
+                Bv.load(sm.B + tt * L::kNP + n0);
+                h = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, h);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) h[i] = fmaf(decay(v.x * (A[i] * 1.44269504f)), hp[i], v.y * Bv[i]);
+                for (int i = 0; i < P; ++i) h.v[i] = fma2(decay2(mul2(d2, A2.v[i])), h.v[i], mul2(dx2, Bv.v[i]));
             }
         }
 #pragma unroll 1
-        for (int sub = L::kTok / K - 1; sub >= 0; --sub) {
-            float a[K][NS], hs[K + 1][NS];
-            load_ns<NS>(sm.start[sub][threadIdx.x], hs[0]);
+        for (int sub = BwdSmem<NS>::kSubs - 1; sub >= 0; --sub) {
+            States<NS> a[K], hs[K + 1];
+            hs[0].load(sm.start[sub][threadIdx.x]);
             float ys[K], gb[K], ra[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
-                const float2 v = *reinterpret_cast<const float2*>(&sm.v[tt][at.cl]);
-                float Bv[NS], Cv[NS];
-                load_ns<NS>(sm.B + tt * L::kNP + n0, Bv);
-                load_ns<NS>(sm.C + tt * L::kNP + n0, Cv);
-                float hp[NS];
-                state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k], hp);
-                float acc = 0.f;
+                const float2 v = sm.dx[tt][at.pos];
+                const F2 d2(v.x), dx2(v.y);
+                States<NS> Bv, Cv;
+                Bv.load(sm.B + tt * L::kNP + n0);
+                Cv.load(sm.C + tt * L::kNP + n0);
+                const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k]);
+                F2 s2(0.f);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    a[k][i] = decay(v.x * (A[i] * 1.44269504f));
-                    hs[k + 1][i] = fmaf(a[k][i], hp[i], v.y * Bv[i]);
-                    acc = fmaf(Cv[i], hs[k + 1][i], acc);
+                for (int i = 0; i < P; ++i) {
+                    a[k].v[i] = decay2(mul2(d2, A2.v[i]));
+                    hs[k + 1].v[i] = fma2(a[k].v[i], hp.v[i], mul2(dx2, Bv.v[i]));
+                    s2 = fma2(Cv.v[i], hs[k + 1].v[i], s2);
                 }
-                ys[k] = acc;
+                ys[k] = s2.x() + s2.y();
             }
 #pragma unroll
             for (int k = K - 1; k >= 0; --k) {
                 const int tt = sub * K + k;
-                const float4 v = sm.v[tt][at.cl];
-                float Bv[NS], Cv[NS], bc[2 * NS];
-                load_ns<NS>(sm.B + tt * L::kNP + n0, Bv);
-                load_ns<NS>(sm.C + tt * L::kNP + n0, Cv);
+                const float2 v = sm.dx[tt][at.pos];
+                const F2 d2(v.x), dx2(v.y), e2(sm.e[tt][at.pos]);
+                States<NS> Bv, Cv;
+                Bv.load(sm.B + tt * L::kNP + n0);
+                Cv.load(sm.C + tt * L::kNP + n0);
                 if (VARLEN && dfin != nullptr) {
                     const int l = sm.marks.last[tt];
-                    if (l >= 0 && at.live) load_user<NS>(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N, g);
+                    if (l >= 0 && at.live) g.load_user(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N);
                 }
-                float hp[NS];
-                state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k], hp);
-                gb[k] = ra[k] = 0.f;
+                const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k]);
+                float bc[2 * NS];
+                F2 gb2(0.f), ra2(0.f);
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    const float G = fmaf(v.z, Cv[i], g[i]);
-                    bc[i] = v.y * G;
-                    bc[NS + i] = v.z * hs[k + 1][i];
-                    gb[k] = fmaf(G, Bv[i], gb[k]);
-                    g[i] = a[k][i] * G;
-                    const float r = g[i] * hp[i];
-                    ra[k] = fmaf(r, A[i], ra[k]);
-                    dA[i] = fmaf(v.x, r, dA[i]);
+                for (int i = 0; i < P; ++i) {
+                    const F2 G = fma2(e2, Cv.v[i], g.v[i]);
+                    mul2(dx2, G).get(bc[2 * i], bc[2 * i + 1]);
+                    mul2(e2, hs[k + 1].v[i]).get(bc[NS + 2 * i], bc[NS + 2 * i + 1]);
+                    gb2 = fma2(G, Bv.v[i], gb2);
+                    g.v[i] = mul2(a[k].v[i], G);
+                    const F2 r = mul2(g.v[i], hp.v[i]);
+                    ra2 = fma2(r, A2.v[i], ra2);
+                    dA.v[i] = fma2(d2, r, dA.v[i]);
                 }
+                gb[k] = gb2.x() + gb2.y();
+                ra[k] = ra2.x() + ra2.y();
                 if (VARLEN) {
                     const int f = sm.marks.first[tt];
                     if (f >= 0) {
-                        if (dinit != nullptr && at.live) store_user<NS>(dinit + ((int64_t)f * p.channels + at.c) * N, n0, N, g);
-#pragma unroll
-                        for (int i = 0; i < NS; ++i) g[i] = 0.f;
+                        if (dinit != nullptr && at.live) g.store_user(dinit + ((int64_t)f * p.channels + at.c) * N, n0, N);
+                        g.zero();
                     }
                 }
                 const int first = sum8<2 * NS>(bc, at.lane);
@@ -628,14 +739,15 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                     sm.dbc[at.warp][tt][(w < NS ? n0 + w : L::kNP + n0 + w - NS)] = bc[i];
                 }
             }
+            __syncwarp();               // the four lanes of a channel are done with its (d, d x) and e of this sub-tile
 #pragma unroll
             for (int k = 0; k < K; k += 4) {
                 const int tt = sub * K + k + at.q;
                 const float y4[4] = {ys[k], ys[k + 1], ys[k + 2], ys[k + 3]}, g4[4] = {gb[k], gb[k + 1], gb[k + 2], gb[k + 3]},
                             r4[4] = {ra[k], ra[k + 1], ra[k + 2], ra[k + 3]};
-                sm.y[tt][at.cl] = sum4(y4, at.q);
-                sm.gB[tt][at.cl] = sum4(g4, at.q);
-                sm.rA[tt][at.cl] = sum4(r4, at.q);
+                sm.e[tt][at.pos] = sum4(y4, at.q);
+                const float sg = sum4(g4, at.q), sr = sum4(r4, at.q);
+                sm.dx[tt][at.pos] = make_float2(sg, sr * 0.69314718f);
             }
         }
         __syncthreads();
@@ -648,44 +760,47 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             part_bc[((((int64_t)at.tile_in_group * p.batch + at.b) * p.len + tb + tt) * p.groups + at.group) * (2 * L::kNP) + w] = s;
         }
         if (t < t1) {
-            BwdRow<T, L::kVPT> r;
-            load_bwd_row<T, NS>(p, at, x, dt, z, dy, t, col, ok, r);
-            float ox[L::kVPT], od[L::kVPT], oz[L::kVPT];
+            BwdShare<T, NS> in;
+            if (ok) in.load(p, at, x, dt, z, dy, t);
+            float ox[V], od[V], oz[V];
 #pragma unroll
-            for (int i = 0; i < L::kVPT; ++i) {
-                const int c = at.c0 + col + i;
-                const float D = p.D != nullptr && c < at.cend ? p.D[c] : 0.f;
-                const float gB = sm.gB[row][col + i];
-                ox[i] = ok ? fmaf(r.d[i], gB, D * r.e[i]) : 0.f;
-                od[i] = ok ? r.slope[i] * fmaf(r.x[i], gB, sm.rA[row][col + i]) : 0.f;
-                if (z != nullptr) {
-                    const float sg = fbla::seq::sigmoid<float>(r.zv[i]);
-                    oz[i] = ok ? r.dy[i] * fmaf(D, r.x[i], sm.y[row][col + i]) * sg * (1.f + r.zv[i] * (1.f - sg)) : 0.f;
+            for (int i = 0; i < V; ++i) {
+                const int s = at.slot(i);
+                ox[i] = od[i] = oz[i] = 0.f;
+                if (ok) {
+                    const float2 v = sm.dx[row][s];
+                    const float xv = in.x.get(i), raw = in.dt.get(i) + sm.bias[s], D = sm.D[s];
+                    const float gate = z != nullptr ? fbla::seq::sigmoid<float>(in.z.get(i)) : 1.f;
+                    const float e = z != nullptr ? in.dy.get(i) * in.z.get(i) * gate : in.dy.get(i);
+                    ox[i] = fmaf(p.softplus ? fbla::seq::softplus(raw) : raw, v.x, D * e);
+                    od[i] = fmaf(xv, v.x, v.y);
+                    if (p.softplus && !(raw > 20.f)) od[i] *= fbla::seq::sigmoid<float>(raw);
+                    if (z != nullptr) oz[i] = in.dy.get(i) * fmaf(D, xv, sm.e[row][s]) * gate * (1.f + in.z.get(i) * (1.f - gate));
+                    sm.dD[i][threadIdx.x] += e * xv;
+                    sm.db[i][threadIdx.x] += od[i];
                 }
-                sm.dD[threadIdx.x][i] += r.e[i] * r.x[i];
-                sm.db[threadIdx.x][i] += od[i];
             }
             const int64_t o = (at.b * p.len + t) * p.channels;
-            store_row<T, L::kVPT>(dx + o, at.c0 + col, at.cend, p.vec, ox);
-            store_row<T, L::kVPT>(ddt + o, at.c0 + col, at.cend, p.vec, od);
-            if (z != nullptr) store_row<T, L::kVPT>(dz + o, at.c0 + col, at.cend, p.vec, oz);
+            store_row<T, V>(dx + o, c, at.cend, p.vec, ox);
+            store_row<T, V>(ddt + o, c, at.cend, p.vec, od);
+            if (z != nullptr) store_row<T, V>(dz + o, c, at.cend, p.vec, oz);
         }
     }
     __syncthreads();
     const int64_t bs = at.b * p.segs + at.seg;
     if ((int)threadIdx.x < kCB && at.c0 + (int)threadIdx.x < at.cend) {
-        const int k = threadIdx.x / L::kVPT, i = threadIdx.x % L::kVPT;
+        const int k = threadIdx.x / V, i = threadIdx.x % V;
         float sD = 0.f, sb = 0.f;
         for (int r = 0; r < L::kTok; ++r) {
-            sD += sm.dD[r * L::kTPR + k][i];
-            sb += sm.db[r * L::kTPR + k][i];
+            sD += sm.dD[i][r * L::kTPR + k];
+            sb += sm.db[i][r * L::kTPR + k];
         }
         part_D[bs * p.channels + at.c0 + threadIdx.x] = sD;
         part_bias[bs * p.channels + at.c0 + threadIdx.x] = sb;
     }
     if (!at.live) return;
-    store_user<NS>(part_A + (bs * p.channels + at.c) * N, n0, N, dA);
-    if (!VARLEN && dinit != nullptr && at.seg == 0) store_user<NS>(dinit + (at.b * p.channels + at.c) * N, n0, N, g);
+    dA.store_user(part_A + (bs * p.channels + at.c) * N, n0, N);
+    if (!VARLEN && dinit != nullptr && at.seg == 0) g.store_user(dinit + (at.b * p.channels + at.c) * N, n0, N);
 }
 
 // dB, dC (batch, token, group, N) from the channel tiles' sums, tiles in order.
@@ -712,25 +827,26 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanParams p,
     float acc = 0.f, xv = 0.f;
     if (at.live) {
         float* hp = state + (at.b * p.channels + at.c) * N;
-        float h[NS], A[NS], Bv[NS], Cv[NS];
-        load_user<NS>(hp, n0, N, h);
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const bool in = n0 + i < N;
-            A[i] = in ? p.A[(int64_t)at.c * N + n0 + i] : 0.f;
-            Bv[i] = in ? to_f<T>(Bm[at.b * p.bs[0] + at.group * p.bs[2] + n0 + i]) : 0.f;
-            Cv[i] = in ? to_f<T>(Cm[at.b * p.cs[0] + at.group * p.cs[2] + n0 + i]) : 0.f;
-        }
+        States<NS> h, A;
+        h.load_user(hp, n0, N);
+        A.load_user(p.A + (int64_t)at.c * N, n0, N);
+        const T* Bp = Bm + at.b * p.bs[0] + at.group * p.bs[2];
+        const T* Cp = Cm + at.b * p.cs[0] + at.group * p.cs[2];
         xv = to_f<T>(x[at.b * p.xs[0] + at.c]);
         float d = to_f<T>(dt[at.b * p.ds[0] + at.c]);
         if (p.bias != nullptr) d += p.bias[at.c];
-        if (p.softplus) d = softplus(d);
+        if (p.softplus) d = fbla::seq::softplus(d);
+        F2 s2(0.f);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            h[i] = fmaf(decay(d * (A[i] * 1.44269504f)), h[i], d * xv * Bv[i]);
-            acc = fmaf(Cv[i], h[i], acc);
+        for (int i = 0; i < NS / 2; ++i) {
+            const int n = n0 + 2 * i;
+            const F2 Bv(n < N ? to_f<T>(Bp[n]) : 0.f, n + 1 < N ? to_f<T>(Bp[n + 1]) : 0.f);
+            const F2 Cv(n < N ? to_f<T>(Cp[n]) : 0.f, n + 1 < N ? to_f<T>(Cp[n + 1]) : 0.f);
+            h.v[i] = fma2(decay2(mul2(F2(d), mul2(A.v[i], F2(1.44269504f)))), h.v[i], mul2(F2(d * xv), Bv));
+            s2 = fma2(Cv, h.v[i], s2);
         }
-        store_user<NS>(hp, n0, N, h);
+        acc = s2.x() + s2.y();
+        h.store_user(hp, n0, N);
     }
     acc += __shfl_xor_sync(0xffffffffu, acc, 1);
     acc += __shfl_xor_sync(0xffffffffu, acc, 2);
@@ -746,7 +862,7 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanParams p,
 
 // ---- host side ------------------------------------------------------------------------------------
 
-int ns_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+int ns_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int np_of(int N) { return 4 * ns_of(N); }
 int tok_of(int N) { return ns_of(N) >= 8 ? 16 : 32; }
 int tiles_per_group(const ScanParams& p) { return (p.channels / p.groups + kCB - 1) / kCB; }
@@ -839,7 +955,7 @@ cudaError_t fill_empty(const ScanParams& p, const float* from, float* to, cudaSt
 template <typename T, int NS, bool VARLEN> cudaError_t run_fwd(const ScanParams& p, const ScanTensors& a, cudaStream_t st) {
     if (cudaError_t e = fill_empty(p, a.init, a.fin, st)) return e;
     if (p.len == 0 || p.batch == 0) return cudaSuccess;
-    using S = FwdSmem<T, NS>;
+    using S = FwdSmem<NS>;
     float* seg_h = a.ws;
     float* seg_d = p.segs > 1 ? a.ws + (int64_t)p.batch * p.segs * p.channels * Tile<NS>::kNP : nullptr;
     if (p.segs > 1) {
@@ -884,13 +1000,13 @@ template <typename T, int NS, bool VARLEN> cudaError_t run_bwd(const ScanParams&
         float* seg_d = seg_g + (int64_t)p.batch * p.segs * p.channels * Tile<NS>::kNP;
         if (p.segs > 1) {
             auto k = scan_bwd_local_kernel<T, NS, VARLEN>;
-            using S = BwdLocalSmem<T, NS>;
+            using S = BwdLocalSmem<NS>;
             if (cudaError_t e = allow_smem(k, sizeof(S))) return e;
             k<<<scan_grid(p), kThreads, sizeof(S), st>>>(p, (const T*)a.dt, (const T*)a.C, (const T*)a.z, (const T*)a.dy, a.dfin, seg_g, seg_d);
             fbla::note_launches(1);
         }
         auto k = scan_bwd_kernel<T, NS, VARLEN>;
-        using S = BwdSmem<T, NS>;
+        using S = BwdSmem<NS>;
         if (cudaError_t e = allow_smem(k, sizeof(S))) return e;
         k<<<scan_grid(p), kThreads, sizeof(S), st>>>(p, (const T*)a.x, (const T*)a.dt, (const T*)a.B, (const T*)a.C, (const T*)a.z, a.init,
                                                      (const T*)a.dy, a.dfin, a.ckpt, seg_g, seg_d, (T*)a.dx, (T*)a.ddt, (T*)a.dz, a.dinit,
@@ -922,7 +1038,6 @@ template <int V> struct Num { static constexpr int value = V; };
 template <typename F> cudaError_t with_shape(int dtype, int N, F f) {
     auto inner = [&](auto* t) {
         switch (ns_of(N)) {
-            case 1: return f(t, Num<1>());
             case 2: return f(t, Num<2>());
             case 4: return f(t, Num<4>());
             default: return f(t, Num<8>());
