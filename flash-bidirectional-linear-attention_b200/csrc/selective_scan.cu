@@ -61,28 +61,25 @@ template <int NS> struct Tile {
     static constexpr int kTPR = kThreads / kTok;        // threads per token then
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// 2^x for the decays of two states, x = d A log2(e).  |x| < 1/8: Taylor polynomial of degree 4 (next term
-// (x ln2)^5 / 5! < 4e-8), 1 exactly at 0, error of the order of one rounding.  Elsewhere the special function
-// unit: measured on B200 it is off by -2e-8 on average between -0.25 and 0, -5e-8 below, so over the 12 steps
-// that a state with x = -1/8 remembers, 2e-7 -- but over the thousands of steps of a slow state an error that
-// always has the same sign would be the largest of all.
+// 2^x for the decays of two states, x = d A log2(e).
+// For x in [-5/64, 0]: 1 + x (ln2 + x (c1 + x c2)), c1 and c2 chosen by minimising the largest error of (2^x - 1) / x
+// over that range with ln2 held fixed: 1.5e-8 at most, a quarter of a rounding, and relative to the steps that a
+// state with such a decay remembers (1 / (x ln2)) an error of the state of 2.7e-7 at most and none for x -> 0.
+// Elsewhere the special function unit: measured on B200 it is off by -2e-8 on average between -0.25 and 0 and by
+// -5e-8 below, which over the 18 steps or fewer that such a state remembers is 4e-7.  Over the thousands of steps
+// of a slow state an error that always has the same sign would be the largest of all, so it is not used there.
+// (A negative x not below -5/64 is, read as an integer, not above that of -5/64.)
 __device__ __forceinline__ F2 decay2(F2 x) {
-    F2 p(9.6181291e-3f);                            // ln2^4 / 4!
-    p = fma2(p, x, F2(5.5504109e-2f));              // ln2^3 / 3!
-    p = fma2(p, x, F2(0.24022651f));                // ln2^2 / 2!
+    F2 p(5.4470904e-2f);
+    p = fma2(p, x, F2(0.24020165f));
     p = fma2(p, x, F2(0.69314718f));
     p = fma2(p, x, F2(1.f));
     float x0, x1, p0, p1;
     x.get(x0, x1);
     p.get(p0, p1);
-    const float e0 = ex2(x0), e1 = ex2(x1);
-    return F2(fabsf(x0) < 0.125f ? p0 : e0, fabsf(x1) < 0.125f ? p1 : e1);
+    asm("{ .reg .pred q; setp.gt.s32 q, %1, 0xBDA00000; @q ex2.approx.ftz.f32 %0, %2; }" : "+f"(p0) : "r"(__float_as_int(x0)), "f"(x0));
+    asm("{ .reg .pred q; setp.gt.s32 q, %1, 0xBDA00000; @q ex2.approx.ftz.f32 %0, %2; }" : "+f"(p1) : "r"(__float_as_int(x1)), "f"(x1));
+    return F2(p0, p1);
 }
 
 // A lane's NS states as pairs
@@ -254,6 +251,17 @@ template <typename T, int NS> struct BCShare {
     }
 };
 
+// Step sizes of two channels, from dt + bias
+__device__ __forceinline__ F2 step2(const ScanParams& p, float r0, float r1) {
+    return p.softplus ? fbla::seq::softplus2(r0, r1) : F2(r0, r1);
+}
+
+__device__ __forceinline__ void load_pairs(const float4* at, F2& a, F2& b) {
+    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(at);
+    a.v = w.x;
+    b.v = w.y;
+}
+
 // Lane q of the four gets the sum over them of v[q].
 __device__ __forceinline__ float sum4(const float (&v)[4], int q) {
     const bool odd = q & 1, high = q & 2;
@@ -270,7 +278,7 @@ template <int NS> __device__ __forceinline__ int64_t seg_at(const ScanParams& p,
 
 template <int NS> struct FwdSmem {
     using L = Tile<NS>;
-    float2 dx[L::kTok][kPad];           // (d, d x)
+    float4 dx[L::kTok][kCB];            // (d, d, d x, d x): as the packed instructions take them
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
     float y[L::kTok][kPad];
     float D[kCB], bias[kCB];            // by slot
@@ -281,7 +289,7 @@ template <int NS> struct FwdSmem {
 // that nothing from before gets through).  Otherwise the outputs.  What the next tile needs from global memory
 // is on its way while a tile is worked on.
 template <typename T, int NS, bool VARLEN, bool LOCAL>
-__global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
+__global__ void __launch_bounds__(kThreads, 2) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
                                                                const T* __restrict__ Bm, const T* __restrict__ Cm,
                                                                const T* __restrict__ z, const float* __restrict__ init,
                                                                T* __restrict__ y, float* __restrict__ fin, float* __restrict__ ckpt,
@@ -351,14 +359,11 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
         cx.zero();
         if (ok) cx = px;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int s = at.slot(i);
-            float d = 0.f;
-            if (ok) {
-                d = pd.get(i) + sm.bias[s];
-                if (p.softplus) d = fbla::seq::softplus(d);
-            }
-            sm.dx[row][s] = make_float2(d, d * cx.get(i));
+        for (int i = 0; i < V; i += 2) {
+            const F2 d = ok ? step2(p, pd.get(i) + sm.bias[at.slot(i)], pd.get(i + 1) + sm.bias[at.slot(i + 1)]) : F2(0.f);
+            const F2 u = mul2(d, F2(cx.get(i), cx.get(i + 1)));
+            sm.dx[row][at.slot(i)] = make_float4(d.x(), d.x(), u.x(), u.x());
+            sm.dx[row][at.slot(i + 1)] = make_float4(d.y(), d.y(), u.y(), u.y());
         }
         pB.template put<VARLEN>(sm.B, sm.marks);
         if (!LOCAL) pC.template put<VARLEN>(sm.C, sm.marks);
@@ -374,13 +379,13 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
             float ys[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 v = sm.dx[tt + k][at.pos];
-                const F2 d2(v.x), dx2(v.y);
+                F2 d2, dx2;
+                load_pairs(&sm.dx[tt + k][at.pos], d2, dx2);
                 States<NS> Bv, Cv;
                 Bv.load(sm.B + (tt + k) * L::kNP + n0);
                 if (!LOCAL) Cv.load(sm.C + (tt + k) * L::kNP + n0);
                 h = state_before<NS, VARLEN>(p, at, sm.marks, tt + k, init, h);
-                if (LOCAL) sum_d += VARLEN && sm.marks.first[tt + k] >= 0 ? INFINITY : v.x;
+                if (LOCAL) sum_d += VARLEN && sm.marks.first[tt + k] >= 0 ? INFINITY : d2.x();
 #pragma unroll
                 for (int i = 0; i < NS / 2; ++i) {
                     h.v[i] = fma2(decay2(mul2(d2, A2.v[i])), h.v[i], mul2(dx2, Bv.v[i]));
@@ -443,19 +448,15 @@ template <typename T, int NS> struct BwdShare {
         load_row<T, V>(dyp + at.b * p.gs[0] + t * p.gs[1], c, at.cend, p.vec, dy);
         if (zp != nullptr) load_row<T, V>(zp + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, z);
     }
-    __device__ __forceinline__ float step(int i, float bias, int soft) const {
-        const float d = dt.get(i) + bias;
-        return soft ? fbla::seq::softplus(d) : d;
-    }
     __device__ __forceinline__ float e(int i, bool gated) const {
         const float g = dy.get(i);
-        return gated ? g * z.get(i) * fbla::seq::sigmoid<float>(z.get(i)) : g;
+        return gated ? g * z.get(i) * fbla::seq::sigmoid<T>(z.get(i)) : g;
     }
 };
 
 template <int NS> struct BwdLocalSmem {
     using L = Tile<NS>;
-    float2 v[L::kTok][kPad];            // (d, e)
+    float4 v[L::kTok][kCB];             // (d, d, e, e)
     float C[L::kTok * L::kNP];
     float bias[kCB];
     Marks marks;
@@ -506,24 +507,27 @@ __global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanP
         bool ok = tb + row < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
 #pragma unroll
-        for (int i = 0; i < L::kVPT; ++i) {
-            const int s = at.slot(i);
-            sm.v[row][s] = ok ? make_float2(next.step(i, sm.bias[s], p.softplus), next.e(i, z != nullptr)) : make_float2(0.f, 0.f);
+        for (int i = 0; i < L::kVPT; i += 2) {
+            const int s = at.slot(i), s1 = at.slot(i + 1);
+            const F2 d = ok ? step2(p, next.dt.get(i) + sm.bias[s], next.dt.get(i + 1) + sm.bias[s1]) : F2(0.f);
+            const float e0 = ok ? next.e(i, z != nullptr) : 0.f, e1 = ok ? next.e(i + 1, z != nullptr) : 0.f;
+            sm.v[row][s] = make_float4(d.x(), d.x(), e0, e0);
+            sm.v[row][s1] = make_float4(d.y(), d.y(), e1, e1);
         }
         pC.template put<VARLEN>(sm.C, sm.marks);
         __syncthreads();
         if (tb > t0) fetch(tb - L::kTok);
 #pragma unroll 4
         for (int tt = L::kTok - 1; tt >= 0; --tt) {
-            const float2 v = sm.v[tt][at.pos];
-            const F2 d2(v.x), e2(v.y);
+            F2 d2, e2;
+            load_pairs(&sm.v[tt][at.pos], d2, e2);
             States<NS> Cv;
             Cv.load(sm.C + tt * L::kNP + n0);
             if (VARLEN && dfin != nullptr) {
                 const int l = sm.marks.last[tt];
                 if (l >= 0 && at.live) g.load_user(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N);
             }
-            sum_d += v.x;
+            sum_d += d2.x();
 #pragma unroll
             for (int i = 0; i < NS / 2; ++i) g.v[i] = mul2(decay2(mul2(d2, A2.v[i])), fma2(e2, Cv.v[i], g.v[i]));
             if (VARLEN && sm.marks.first[tt] >= 0) {
@@ -566,8 +570,8 @@ template <int M> __device__ __forceinline__ int sum8(float (&v)[M], int lane) {
 template <int NS> struct BwdSmem {
     using L = Tile<NS>;
     static constexpr int kSubs = L::kTok / L::kSub;
-    float2 dx[L::kTok][kPad];                       // (d, d x); behind the reverse pass of a sub-tile (sum G B, sum A r)
-    float e[L::kTok][kPad];                         // e; then s = sum C h
+    float4 dx[L::kTok][kCB];                        // (d, d, d x, d x); behind a sub-tile's reverse pass (d, s, sum G B, sum A r)
+    float e[L::kTok][kPad];
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
     float start[kSubs][kThreads][NS];               // each thread's states at the starts of the sub-tiles
     float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its eight channels
@@ -648,11 +652,17 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             bc.load(Cm, p.cs, p, at, tb, t1);
             bc.template put<VARLEN>(sm.C, sm.marks);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int s = at.slot(i);
-                const float d = ok ? in.step(i, sm.bias[s], p.softplus) : 0.f;
-                sm.dx[row][s] = make_float2(d, ok ? d * in.x.get(i) : 0.f);
+            for (int i = 0; i < V; i += 2) {
+                const int s = at.slot(i), s1 = at.slot(i + 1);
+                F2 d(0.f), u(0.f);
+                if (ok) {
+                    d = step2(p, in.dt.get(i) + sm.bias[s], in.dt.get(i + 1) + sm.bias[s1]);
+                    u = mul2(d, F2(in.x.get(i), in.x.get(i + 1)));
+                }
+                sm.dx[row][s] = make_float4(d.x(), d.x(), u.x(), u.x());
+                sm.dx[row][s1] = make_float4(d.y(), d.y(), u.y(), u.y());
                 sm.e[row][s] = ok ? in.e(i, z != nullptr) : 0.f;
+                sm.e[row][s1] = ok ? in.e(i + 1, z != nullptr) : 0.f;
             }
         }
         __syncthreads();
@@ -664,8 +674,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
-                const float2 v = sm.dx[tt][at.pos];
-                const F2 d2(v.x), dx2(v.y);
+                F2 d2, dx2;
+                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
                 States<NS> Bv;
                 Bv.load(sm.B + tt * L::kNP + n0);
                 h = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, h);
@@ -681,8 +691,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
-                const float2 v = sm.dx[tt][at.pos];
-                const F2 d2(v.x), dx2(v.y);
+                F2 d2, dx2;
+                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
                 States<NS> Bv, Cv;
                 Bv.load(sm.B + tt * L::kNP + n0);
                 Cv.load(sm.C + tt * L::kNP + n0);
@@ -699,8 +709,9 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
 #pragma unroll
             for (int k = K - 1; k >= 0; --k) {
                 const int tt = sub * K + k;
-                const float2 v = sm.dx[tt][at.pos];
-                const F2 d2(v.x), dx2(v.y), e2(sm.e[tt][at.pos]);
+                F2 d2, dx2;
+                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
+                const F2 e2(sm.e[tt][at.pos]);
                 States<NS> Bv, Cv;
                 Bv.load(sm.B + tt * L::kNP + n0);
                 Cv.load(sm.C + tt * L::kNP + n0);
@@ -739,15 +750,16 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                     sm.dbc[at.warp][tt][(w < NS ? n0 + w : L::kNP + n0 + w - NS)] = bc[i];
                 }
             }
-            __syncwarp();               // the four lanes of a channel are done with its (d, d x) and e of this sub-tile
+            __syncwarp();               // the four lanes of a channel are done with its (d, d x) of this sub-tile
 #pragma unroll
             for (int k = 0; k < K; k += 4) {
                 const int tt = sub * K + k + at.q;
                 const float y4[4] = {ys[k], ys[k + 1], ys[k + 2], ys[k + 3]}, g4[4] = {gb[k], gb[k + 1], gb[k + 2], gb[k + 3]},
                             r4[4] = {ra[k], ra[k + 1], ra[k + 2], ra[k + 3]};
-                sm.e[tt][at.pos] = sum4(y4, at.q);
-                const float sg = sum4(g4, at.q), sr = sum4(r4, at.q);
-                sm.dx[tt][at.pos] = make_float2(sg, sr * 0.69314718f);
+                const float sy = sum4(y4, at.q), sg = sum4(g4, at.q), sr = sum4(r4, at.q);
+                float4& o = sm.dx[tt][at.pos];
+                o.y = sy;
+                *reinterpret_cast<float2*>(&o.z) = make_float2(sg, sr * 0.69314718f);
             }
         }
         __syncthreads();
@@ -768,14 +780,18 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                 const int s = at.slot(i);
                 ox[i] = od[i] = oz[i] = 0.f;
                 if (ok) {
-                    const float2 v = sm.dx[row][s];
-                    const float xv = in.x.get(i), raw = in.dt.get(i) + sm.bias[s], D = sm.D[s];
-                    const float gate = z != nullptr ? fbla::seq::sigmoid<float>(in.z.get(i)) : 1.f;
-                    const float e = z != nullptr ? in.dy.get(i) * in.z.get(i) * gate : in.dy.get(i);
-                    ox[i] = fmaf(p.softplus ? fbla::seq::softplus(raw) : raw, v.x, D * e);
-                    od[i] = fmaf(xv, v.x, v.y);
-                    if (p.softplus && !(raw > 20.f)) od[i] *= fbla::seq::sigmoid<float>(raw);
-                    if (z != nullptr) oz[i] = in.dy.get(i) * fmaf(D, xv, sm.e[row][s]) * gate * (1.f + in.z.get(i) * (1.f - gate));
+                    const float4 v = sm.dx[row][s];         // d, s, sum G B, sum A r
+                    const float xv = in.x.get(i), D = sm.D[s], e = sm.e[row][s];
+                    ox[i] = fmaf(v.x, v.z, D * e);
+                    od[i] = fmaf(xv, v.z, v.w);
+                    if (p.softplus) {
+                        const float raw = in.dt.get(i) + sm.bias[s];
+                        if (!(raw > 20.f)) od[i] *= fbla::seq::sigmoid<T>(raw);
+                    }
+                    if (z != nullptr) {
+                        const float zv = in.z.get(i), gate = fbla::seq::sigmoid<T>(zv);
+                        oz[i] = in.dy.get(i) * fmaf(D, xv, v.y) * gate * (1.f + zv * (1.f - gate));
+                    }
                     sm.dD[i][threadIdx.x] += e * xv;
                     sm.db[i][threadIdx.x] += od[i];
                 }

@@ -82,27 +82,6 @@ __device__ __forceinline__ float exp_of(float x) { return x != x ? x : exp_full(
 template <typename T> __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 template <> __device__ __forceinline__ float sigmoid<float>(float x) { return __frcp_rn(1.f + exp_of(-x)); }
 
-// log(1 + e^v): max(v, 0) + log1p(w) with w = e^-|v| in (0, 1], and log1p(w) = 2 atanh(w / (2 + w)) as its
-// series in s = w / (2 + w) <= 1/3 (the first term left out is s^14 / 15 = 1.4e-8 relative).  e^-|v| is the special
-// function unit's 2^x; what rounding |v| log2(e) loses (2^-24 of up to 150) comes back as a factor.  About 3
-// units in the last place; two special functions and twenty other instructions.
-__device__ __forceinline__ float softplus(float v) {
-    const float m = !(v <= 0.f) ? v : 0.f;          // a NaN stays
-    const float a = fminf(fabsf(v), 104.f);         // e^-104 is 0 in fp32
-    const float x = a * -1.44269504f;
-    const float lost = fmaf(a, -1.44269504f, -x) + a * -1.92596299e-8f;
-    const float e = exp2f(x), w = fmaf(e * 0.69314718f, lost, e);
-    const float s = __fdividef(w, 2.f + w), t = s * s;
-    float p = 2.f / 13.f;
-    p = fmaf(p, t, 2.f / 11.f);
-    p = fmaf(p, t, 2.f / 9.f);
-    p = fmaf(p, t, 2.f / 7.f);
-    p = fmaf(p, t, 2.f / 5.f);
-    p = fmaf(p, t, 2.f / 3.f);
-    p = fmaf(p, t, 2.f);
-    return fmaf(p, s, m);
-}
-
 // Two fp32 values in one 64-bit register: one instruction for two multiply-adds.  The rate of the multiply-add
 // units is the same (128 per clock and SM measured either way), half of the issue slots are left to others.
 struct F2 {
@@ -124,6 +103,42 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
     asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// log(1 + e^v) of two values: max(v, 0) + log1p(w) with w = e^-|v| in (0, 1], and log1p(w) = 2 atanh(w / (2 + w))
+// as its series in s = w / (2 + w) <= 1/3 (the first term left out is s^14 / 15 = 1.4e-8 relative).  e^-|v| is the
+// special function unit's 2^x; what rounding |v| log2(e) loses (2^-24 of up to 150) comes back as a factor.
+// About 3 units in the last place.
+__device__ __forceinline__ F2 softplus2(float v0, float v1) {
+    const F2 m(!(v0 <= 0.f) ? v0 : 0.f, !(v1 <= 0.f) ? v1 : 0.f);      // a NaN stays
+    const F2 a(fminf(fabsf(v0), 104.f), fminf(fabsf(v1), 104.f));      // e^-104 is 0 in fp32
+    const F2 x = mul2(a, F2(1.44269504f));
+    F2 lost = fma2(a, F2(-1.44269504f), x);
+    lost = fma2(a, F2(-1.92596299e-8f), lost);
+    const F2 e(ex2(-x.x()), ex2(-x.y()));
+    const F2 w = fma2(mul2(e, F2(0.69314718f)), lost, e);
+    const F2 den = fma2(w, F2(1.f), F2(2.f));
+    const F2 s = mul2(w, F2(rcp(den.x()), rcp(den.y()))), t = mul2(s, s);
+    F2 p(2.f / 13.f);
+    p = fma2(p, t, F2(2.f / 11.f));
+    p = fma2(p, t, F2(2.f / 9.f));
+    p = fma2(p, t, F2(2.f / 7.f));
+    p = fma2(p, t, F2(2.f / 5.f));
+    p = fma2(p, t, F2(2.f / 3.f));
+    p = fma2(p, t, F2(2.f));
+    return fma2(p, s, m);
+}
+__device__ __forceinline__ float softplus(float v) { return softplus2(v, 0.f).x(); }
 
 // ---- packed sequences -----------------------------------------------------------------------------
 // Sequence s owns tokens [cu[s], cu[s+1]).
