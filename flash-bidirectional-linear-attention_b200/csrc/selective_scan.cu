@@ -12,15 +12,16 @@
 // to 1 is where an error of the exponential would add up over the steps that a state remembers, so those
 // come from a polynomial that is exact at 0 (see decay()).
 //
-// Layout: four lanes share a channel, each holding N/4 states in registers, so a warp owns 8 channels and
-// a CTA 64; the tokens go by in tiles whose x, dt (turned into d and d x once per channel, not once per
-// lane) and B, C are staged in shared memory.  The sum over the four lanes is a transposed butterfly over
-// four tokens: three shuffles for four results.
+// Layout: four lanes share two channels, each lane holding N/4 states of both in registers, so a warp owns 16
+// channels and a CTA of four warps 64; the tokens go by in tiles whose x, dt (turned into d and d x once per
+// channel, not once per lane) and B, C are staged in shared memory.  Two channels per lane because what a lane
+// reads of B and C counts: shared memory delivers 128 bytes per clock to the registers of an SM whether lanes
+// read the same address or not, and with one channel per lane those reads took as long as the arithmetic.  The
+// sum over the four lanes is a transposed butterfly over four tokens: three shuffles for four results.
 // A CTA walks over one segment of the tokens.  With few channels the tokens are cut into several
 // segments: a first pass forms each segment's own end state (from zero) and its total decay, which is
 // exp(A sum d); the main pass starts from the combination of the segments before it.  The backward pass
 // does the same from the other end.
-#include <cfloat>
 #include <type_traits>
 
 #include "seq_common.cuh"
@@ -35,11 +36,11 @@ using fbla::seq::F2;
 using fbla::seq::fma2;
 using fbla::seq::mul2;
 
-constexpr int kCB = 64;             // channels of a CTA
-constexpr int kThreads = 4 * kCB;
+constexpr int kCB = 64;                 // channels of a CTA
+constexpr int kThreads = 2 * kCB;       // four lanes for two channels
 constexpr int kWarps = kThreads / 32;
-constexpr int kPad = kCB + 8;       // row of a per-token, per-channel array: the four lanes of a channel write four rows
-                                    // at once, 8 banks apart
+constexpr int kRow4 = kCB / 2 + 4;      // row of 16-byte slots (two channels each): 64 bytes of padding
+constexpr int kRow2 = kCB / 2 + 4;      // row of 8-byte slots: 32 bytes of padding
 
 struct ScanParams {
     int batch, channels, states, groups, softplus, num_seqs;
@@ -137,12 +138,13 @@ template <int NS> struct States {
 
 // Where this CTA and lane stand.
 template <int NS> struct Place {
+    using L = Tile<NS>;
     int64_t b;
     int seg, group, c0, cend;   // c0: first channel of the CTA, cend: end of its group
     int tile_in_group;
     int warp, lane, q;          // q: which states the lane holds
-    int pos, c;                 // the lane's channel: its position in a row of shared memory, its number
-    bool live;
+    int slot, c;                // the lane's two channels: their slot in a row of shared memory, the number of the first
+    bool live[2];
     __device__ __forceinline__ Place(const ScanParams& p) {
         const int cpg = p.channels / p.groups, tpg = (cpg + kCB - 1) / kCB;
         b = blockIdx.z;
@@ -154,15 +156,17 @@ template <int NS> struct Place {
         warp = threadIdx.x >> 5;
         lane = threadIdx.x & 31;
         q = lane & 3;
-        pos = warp * 8 + (lane >> 2);
-        c = c0 + (pos % Tile<NS>::kTPR) * Tile<NS>::kVPT + pos / Tile<NS>::kTPR;
-        live = c < cend;
+        slot = warp * 8 + (lane >> 2);
+        c = c0 + (slot % L::kTPR) * L::kVPT + slot / L::kTPR * 2;
+        live[0] = c < cend;
+        live[1] = c + 1 < cend;
     }
-    // When a tile is loaded or stored a thread has kVPT consecutive channels of one token, and the i-th of them
-    // lies at slot(i): threads next to each other write next to each other, and so read the lanes of a warp.
-    __device__ __forceinline__ static int row() { return threadIdx.x / Tile<NS>::kTPR; }
-    __device__ __forceinline__ static int col() { return threadIdx.x % Tile<NS>::kTPR * Tile<NS>::kVPT; }
-    __device__ __forceinline__ static int slot(int i) { return i * Tile<NS>::kTPR + threadIdx.x % Tile<NS>::kTPR; }
+    // When a tile is loaded or stored a thread has kVPT consecutive channels of one token; the channels 2 i and
+    // 2 i + 1 of them lie at slot(i): threads next to each other write next to each other, and so read the lanes
+    // of a warp.
+    __device__ __forceinline__ static int row() { return threadIdx.x / L::kTPR; }
+    __device__ __forceinline__ static int col() { return threadIdx.x % L::kTPR * L::kVPT; }
+    __device__ __forceinline__ static int slot_of(int i) { return i * L::kTPR + threadIdx.x % L::kTPR; }
 };
 
 // Packed sequences: what happens at a token of the tile.
@@ -191,13 +195,13 @@ __device__ __forceinline__ void fill_marks(const ScanParams& p, Marks* m, int64_
 // The state that token `tt` of the tile continues from: that of the token before it, unless a sequence begins.
 template <int NS, bool VARLEN>
 __device__ __forceinline__ States<NS> state_before(const ScanParams& p, const Place<NS>& at, const Marks& m, int tt, const float* init,
-                                                   const States<NS>& h) {
+                                                   const States<NS>& h, int ch) {
     States<NS> r = h;
     if (VARLEN) {
         const int f = m.first[tt];
         if (f >= 0) {
             r.zero();
-            if (init != nullptr && at.live) r.load_user(init + ((int64_t)f * p.channels + at.c) * p.states, at.q * NS, p.states);
+            if (init != nullptr && at.live[ch]) r.load_user(init + ((int64_t)f * p.channels + at.c + ch) * p.states, at.q * NS, p.states);
         }
     }
     return r;
@@ -256,12 +260,6 @@ __device__ __forceinline__ F2 step2(const ScanParams& p, float r0, float r1) {
     return p.softplus ? fbla::seq::softplus2(r0, r1) : F2(r0, r1);
 }
 
-__device__ __forceinline__ void load_pairs(const float4* at, F2& a, F2& b) {
-    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(at);
-    a.v = w.x;
-    b.v = w.y;
-}
-
 // Lane q of the four gets the sum over them of v[q].
 __device__ __forceinline__ float sum4(const float (&v)[4], int q) {
     const bool odd = q & 1, high = q & 2;
@@ -271,25 +269,63 @@ __device__ __forceinline__ float sum4(const float (&v)[4], int q) {
     return (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
 }
 
+// A log2(e) of the lane's two channels
+template <int NS> __device__ __forceinline__ void load_rates(const ScanParams& p, const Place<NS>& at, States<NS> (&A2)[2]) {
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        A2[ch].zero();
+        if (at.live[ch]) A2[ch].load_user(p.A + (int64_t)(at.c + ch) * p.states, at.q * NS, p.states);
+#pragma unroll
+        for (int i = 0; i < NS / 2; ++i) A2[ch].v[i] = mul2(A2[ch].v[i], F2(1.44269504f));
+    }
+}
+
 // Workspace of the segmented passes: [batch][segs][channels][kNP] states, then [batch][segs][channels] sums of d.
 template <int NS> __device__ __forceinline__ int64_t seg_at(const ScanParams& p, int64_t b, int seg, int c) {
     return (b * p.segs + seg) * p.channels + c;
 }
 
+// v <- own state of segment j + (its decay) v, for the lane's two channels
+template <int NS>
+__device__ __forceinline__ void add_segment(const ScanParams& p, const Place<NS>& at, int j, const float* seg_v, const float* seg_d,
+                                            const States<NS> (&A2)[2], States<NS> (&v)[2]) {
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        if (!at.live[ch]) continue;
+        const int64_t k = seg_at<NS>(p, at.b, j, at.c + ch);
+        const float sd = seg_d[k];
+        States<NS> own;
+        own.load(seg_v + k * Tile<NS>::kNP + at.q * NS);
+#pragma unroll
+        for (int i = 0; i < NS / 2; ++i)
+            v[ch].v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2[ch].v[i])), v[ch].v[i], own.v[i]);
+    }
+}
+
 template <int NS> struct FwdSmem {
     using L = Tile<NS>;
-    float4 dx[L::kTok][kCB];            // (d, d, d x, d x): as the packed instructions take them
+    float4 dx[L::kTok][kRow4];          // per two channels (d, d x, d, d x)
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
-    float y[L::kTok][kPad];
-    float D[kCB], bias[kCB];            // by slot
+    float2 y[L::kTok][kRow2];
+    float2 D[kCB / 2], bias[kCB / 2];   // by slot
     Marks marks;
 };
+
+template <int NS> __device__ __forceinline__ void load_per_channel(const ScanParams& p, const Place<NS>& at, const float* src, float2* dst) {
+    if (at.row() != 0) return;
+    const int c = at.c0 + at.col();
+#pragma unroll
+    for (int i = 0; i < Tile<NS>::kVPT / 2; ++i) {
+        const int k = c + 2 * i;
+        dst[at.slot_of(i)] = make_float2(src != nullptr && k < at.cend ? src[k] : 0.f, src != nullptr && k + 1 < at.cend ? src[k + 1] : 0.f);
+    }
+}
 
 // LOCAL: end state of the segment from zero, and the sum of d (infinite when a sequence begins inside, so
 // that nothing from before gets through).  Otherwise the outputs.  What the next tile needs from global memory
 // is on its way while a tile is worked on.
 template <typename T, int NS, bool VARLEN, bool LOCAL>
-__global__ void __launch_bounds__(kThreads, 2) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
+__global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
                                                                const T* __restrict__ Bm, const T* __restrict__ Cm,
                                                                const T* __restrict__ z, const float* __restrict__ init,
                                                                T* __restrict__ y, float* __restrict__ fin, float* __restrict__ ckpt,
@@ -303,35 +339,19 @@ __global__ void __launch_bounds__(kThreads, 2) scan_fwd_kernel(const ScanParams 
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
 
-    States<NS> A2, h;
-    float sum_d = 0.f;
-    A2.zero();
-    h.zero();
-    if (at.live) {
-        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
+    States<NS> A2[2], h[2];
+    float sum_d[2] = {0.f, 0.f};
+    load_rates<NS>(p, at, A2);
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
-        if (!LOCAL) {
-            if (!VARLEN && init != nullptr) h.load_user(init + (at.b * p.channels + at.c) * N, n0, N);
-            for (int j = 0; j < at.seg; ++j) {
-                const int64_t k = seg_at<NS>(p, at.b, j, at.c);
-                const float sd = seg_d[k];
-                States<NS> own;
-                own.load(seg_h + k * L::kNP + n0);
-#pragma unroll
-                for (int i = 0; i < NS / 2; ++i)
-                    h.v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2.v[i])), h.v[i], own.v[i]);
-            }
-        }
+    for (int ch = 0; ch < 2; ++ch) {
+        h[ch].zero();
+        if (!LOCAL && !VARLEN && init != nullptr && at.live[ch]) h[ch].load_user(init + (at.b * p.channels + at.c + ch) * N, n0, N);
     }
+    if (!LOCAL)
+        for (int j = 0; j < at.seg; ++j) add_segment<NS>(p, at, j, seg_h, seg_d, A2, h);
     const int row = at.row(), c = at.c0 + at.col();     // when loading or storing
-    if (row == 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            sm.D[at.slot(i)] = p.D != nullptr && c + i < at.cend ? p.D[c + i] : 0.f;
-            sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
-        }
-    }
+    load_per_channel<NS>(p, at, p.D, sm.D);
+    load_per_channel<NS>(p, at, p.bias, sm.bias);
     const int64_t ntiles = (p.len + L::kTok - 1) / L::kTok;
 
     Pack<T, V> px, pd;
@@ -359,11 +379,11 @@ __global__ void __launch_bounds__(kThreads, 2) scan_fwd_kernel(const ScanParams 
         cx.zero();
         if (ok) cx = px;
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const F2 d = ok ? step2(p, pd.get(i) + sm.bias[at.slot(i)], pd.get(i + 1) + sm.bias[at.slot(i + 1)]) : F2(0.f);
-            const F2 u = mul2(d, F2(cx.get(i), cx.get(i + 1)));
-            sm.dx[row][at.slot(i)] = make_float4(d.x(), d.x(), u.x(), u.x());
-            sm.dx[row][at.slot(i + 1)] = make_float4(d.y(), d.y(), u.y(), u.y());
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 bias = sm.bias[at.slot_of(i)];
+            const F2 d = ok ? step2(p, pd.get(2 * i) + bias.x, pd.get(2 * i + 1) + bias.y) : F2(0.f);
+            const F2 u = mul2(d, F2(cx.get(2 * i), cx.get(2 * i + 1)));
+            sm.dx[row][at.slot_of(i)] = make_float4(d.x(), u.x(), d.y(), u.y());
         }
         pB.template put<VARLEN>(sm.B, sm.marks);
         if (!LOCAL) pC.template put<VARLEN>(sm.C, sm.marks);
@@ -372,57 +392,71 @@ __global__ void __launch_bounds__(kThreads, 2) scan_fwd_kernel(const ScanParams 
         if (tb + L::kTok < t1) fetch(tb + L::kTok);
         if (!LOCAL) {
             if (z != nullptr && t < t1) load_row<T, V>(z + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, cz);
-            if (ckpt != nullptr && at.live) h.store(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0));
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch)
+                if (ckpt != nullptr && at.live[ch])
+                    h[ch].store(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0));
         }
-#pragma unroll 2
+#pragma unroll 1
         for (int tt = 0; tt < L::kTok; tt += 4) {
-            float ys[4];
+            float ys[2][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                F2 d2, dx2;
-                load_pairs(&sm.dx[tt + k][at.pos], d2, dx2);
+                const float4 v = sm.dx[tt + k][at.slot];
                 States<NS> Bv, Cv;
                 Bv.load(sm.B + (tt + k) * L::kNP + n0);
                 if (!LOCAL) Cv.load(sm.C + (tt + k) * L::kNP + n0);
-                h = state_before<NS, VARLEN>(p, at, sm.marks, tt + k, init, h);
-                if (LOCAL) sum_d += VARLEN && sm.marks.first[tt + k] >= 0 ? INFINITY : d2.x();
 #pragma unroll
-                for (int i = 0; i < NS / 2; ++i) {
-                    h.v[i] = fma2(decay2(mul2(d2, A2.v[i])), h.v[i], mul2(dx2, Bv.v[i]));
-                }
-                if (!LOCAL) {
-                    F2 s2 = mul2(Cv.v[0], h.v[0]);
+                for (int ch = 0; ch < 2; ++ch) {
+                    const float d = ch ? v.z : v.x;
+                    const F2 d2(d), dx2(ch ? v.w : v.y);
+                    h[ch] = state_before<NS, VARLEN>(p, at, sm.marks, tt + k, init, h[ch], ch);
+                    if (LOCAL) sum_d[ch] += VARLEN && sm.marks.first[tt + k] >= 0 ? INFINITY : d;
+                    F2 s2(0.f);
 #pragma unroll
-                    for (int i = 1; i < NS / 2; ++i) s2 = fma2(Cv.v[i], h.v[i], s2);
-                    ys[k] = s2.x() + s2.y();
-                }
-                if (VARLEN && !LOCAL && fin != nullptr) {
-                    const int l = sm.marks.last[tt + k];
-                    if (l >= 0 && at.live) h.store_user(fin + ((int64_t)l * p.channels + at.c) * N, n0, N);
+                    for (int i = 0; i < NS / 2; ++i) {
+                        h[ch].v[i] = fma2(decay2(mul2(d2, A2[ch].v[i])), h[ch].v[i], mul2(dx2, Bv.v[i]));
+                        if (!LOCAL) s2 = i == 0 ? mul2(Cv.v[i], h[ch].v[i]) : fma2(Cv.v[i], h[ch].v[i], s2);
+                    }
+                    ys[ch][k] = s2.x() + s2.y();
+                    if (VARLEN && !LOCAL && fin != nullptr) {
+                        const int l = sm.marks.last[tt + k];
+                        if (l >= 0 && at.live[ch]) h[ch].store_user(fin + ((int64_t)l * p.channels + at.c + ch) * N, n0, N);
+                    }
                 }
             }
-            if (!LOCAL) sm.y[tt + at.q][at.pos] = sum4(ys, at.q);
+            if (!LOCAL) {
+                const float y0 = sum4(ys[0], at.q), y1 = sum4(ys[1], at.q);
+                sm.y[tt + at.q][at.slot] = make_float2(y0, y1);
+            }
         }
         __syncthreads();
         if (!LOCAL && t < t1) {
             float out[V];
 #pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 s = sm.y[row][at.slot_of(i)], D = sm.D[at.slot_of(i)];
+                out[2 * i] = fmaf(D.x, cx.get(2 * i), s.x);
+                out[2 * i + 1] = fmaf(D.y, cx.get(2 * i + 1), s.y);
+            }
+#pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int s = at.slot(i);
-                float v = fmaf(sm.D[s], cx.get(i), sm.y[row][s]);
-                if (z != nullptr) v *= cz.get(i) * fbla::seq::sigmoid<T>(cz.get(i));
-                out[i] = ok ? v : 0.f;
+                if (z != nullptr) out[i] *= cz.get(i) * fbla::seq::sigmoid<T>(cz.get(i));
+                if (!ok) out[i] = 0.f;
             }
             store_row<T, V>(y + (at.b * p.len + t) * p.channels, c, at.cend, p.vec, out);
         }
     }
-    if (!at.live) return;
-    if (LOCAL) {
-        const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c);
-        h.store(seg_h + k * L::kNP + n0);
-        if (at.q == 0) seg_d[k] = sum_d;
-    } else if (!VARLEN && fin != nullptr && at.seg == p.segs - 1) {
-        h.store_user(fin + (at.b * p.channels + at.c) * N, n0, N);
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        if (!at.live[ch]) continue;
+        if (LOCAL) {
+            const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c + ch);
+            h[ch].store(seg_h + k * L::kNP + n0);
+            if (at.q == 0) seg_d[k] = sum_d[ch];
+        } else if (!VARLEN && fin != nullptr && at.seg == p.segs - 1) {
+            h[ch].store_user(fin + (at.b * p.channels + at.c + ch) * N, n0, N);
+        }
     }
 }
 
@@ -456,9 +490,9 @@ template <typename T, int NS> struct BwdShare {
 
 template <int NS> struct BwdLocalSmem {
     using L = Tile<NS>;
-    float4 v[L::kTok][kCB];             // (d, d, e, e)
+    float4 v[L::kTok][kRow4];           // per two channels (d, e, d, e)
     float C[L::kTok * L::kNP];
-    float bias[kCB];
+    float2 bias[kCB / 2];
     Marks marks;
 };
 
@@ -475,21 +509,17 @@ __global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanP
     if (at.seg == 0) return;            // nothing comes before it
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
-    States<NS> A2, g;
-    float sum_d = 0.f;
-    A2.zero();
-    g.zero();
-    if (at.live) {
-        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
+    States<NS> A2[2], g[2];
+    float sum_d[2] = {0.f, 0.f};
+    load_rates<NS>(p, at, A2);
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
-        if (!VARLEN && dfin != nullptr && at.seg == p.segs - 1) g.load_user(dfin + (at.b * p.channels + at.c) * N, n0, N);
+    for (int ch = 0; ch < 2; ++ch) {
+        g[ch].zero();
+        if (!VARLEN && dfin != nullptr && at.live[ch] && at.seg == p.segs - 1)
+            g[ch].load_user(dfin + (at.b * p.channels + at.c + ch) * N, n0, N);
     }
-    const int row = at.row(), c = at.c0 + at.col();
-    if (row == 0) {
-#pragma unroll
-        for (int i = 0; i < L::kVPT; ++i) sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
-    }
+    load_per_channel<NS>(p, at, p.bias, sm.bias);
+    const int row = at.row();
     BwdShare<T, NS> next;
     BCShare<T, NS> pC;
     auto fetch = [&](int64_t tb) {
@@ -507,39 +537,47 @@ __global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanP
         bool ok = tb + row < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
 #pragma unroll
-        for (int i = 0; i < L::kVPT; i += 2) {
-            const int s = at.slot(i), s1 = at.slot(i + 1);
-            const F2 d = ok ? step2(p, next.dt.get(i) + sm.bias[s], next.dt.get(i + 1) + sm.bias[s1]) : F2(0.f);
-            const float e0 = ok ? next.e(i, z != nullptr) : 0.f, e1 = ok ? next.e(i + 1, z != nullptr) : 0.f;
-            sm.v[row][s] = make_float4(d.x(), d.x(), e0, e0);
-            sm.v[row][s1] = make_float4(d.y(), d.y(), e1, e1);
+        for (int i = 0; i < L::kVPT / 2; ++i) {
+            const float2 bias = sm.bias[at.slot_of(i)];
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (ok) {
+                const F2 d = step2(p, next.dt.get(2 * i) + bias.x, next.dt.get(2 * i + 1) + bias.y);
+                v = make_float4(d.x(), next.e(2 * i, z != nullptr), d.y(), next.e(2 * i + 1, z != nullptr));
+            }
+            sm.v[row][at.slot_of(i)] = v;
         }
         pC.template put<VARLEN>(sm.C, sm.marks);
         __syncthreads();
         if (tb > t0) fetch(tb - L::kTok);
 #pragma unroll 4
         for (int tt = L::kTok - 1; tt >= 0; --tt) {
-            F2 d2, e2;
-            load_pairs(&sm.v[tt][at.pos], d2, e2);
+            const float4 v = sm.v[tt][at.slot];
             States<NS> Cv;
             Cv.load(sm.C + tt * L::kNP + n0);
-            if (VARLEN && dfin != nullptr) {
-                const int l = sm.marks.last[tt];
-                if (l >= 0 && at.live) g.load_user(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N);
-            }
-            sum_d += d2.x();
 #pragma unroll
-            for (int i = 0; i < NS / 2; ++i) g.v[i] = mul2(decay2(mul2(d2, A2.v[i])), fma2(e2, Cv.v[i], g.v[i]));
-            if (VARLEN && sm.marks.first[tt] >= 0) {
-                sum_d = INFINITY;
-                g.zero();
+            for (int ch = 0; ch < 2; ++ch) {
+                const F2 d2(ch ? v.z : v.x), e2(ch ? v.w : v.y);
+                if (VARLEN && dfin != nullptr) {
+                    const int l = sm.marks.last[tt];
+                    if (l >= 0 && at.live[ch]) g[ch].load_user(dfin + ((int64_t)l * p.channels + at.c + ch) * N, n0, N);
+                }
+                sum_d[ch] += d2.x();
+#pragma unroll
+                for (int i = 0; i < NS / 2; ++i) g[ch].v[i] = mul2(decay2(mul2(d2, A2[ch].v[i])), fma2(e2, Cv.v[i], g[ch].v[i]));
+                if (VARLEN && sm.marks.first[tt] >= 0) {
+                    sum_d[ch] = INFINITY;
+                    g[ch].zero();
+                }
             }
         }
     }
-    if (!at.live) return;
-    const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c);
-    g.store(seg_g + k * L::kNP + n0);
-    if (at.q == 0) seg_d[k] = sum_d;
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        if (!at.live[ch]) continue;
+        const int64_t k = seg_at<NS>(p, at.b, at.seg, at.c + ch);
+        g[ch].store(seg_g + k * L::kNP + n0);
+        if (at.q == 0) seg_d[k] = sum_d[ch];
+    }
 }
 
 // Sums over the eight channels of a warp (lane bits 2, 3, 4) of the M values each lane holds: halving
@@ -570,13 +608,14 @@ template <int M> __device__ __forceinline__ int sum8(float (&v)[M], int lane) {
 template <int NS> struct BwdSmem {
     using L = Tile<NS>;
     static constexpr int kSubs = L::kTok / L::kSub;
-    float4 dx[L::kTok][kCB];                        // (d, d, d x, d x); behind a sub-tile's reverse pass (d, s, sum G B, sum A r)
-    float e[L::kTok][kPad];
+    float4 dx[L::kTok][kRow4];                      // per two channels (d, d x, d, d x); behind its reverse pass sum G B for d x
+    float2 e[L::kTok][kRow2];                       // e; behind the reverse pass sum A r
+    float2 y[L::kTok][kRow2];                       // s = sum C h
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
-    float start[kSubs][kThreads][NS];               // each thread's states at the starts of the sub-tiles
-    float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its eight channels
+    float start[kSubs][2][kThreads][NS];            // each thread's states at the starts of the sub-tiles
+    float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its channels
     float dD[L::kVPT][kThreads], db[L::kVPT][kThreads];
-    float D[kCB], bias[kCB];
+    float2 D[kCB / 2], bias[kCB / 2];
     Marks marks;
 };
 
@@ -601,33 +640,20 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
     const int64_t ntiles = (p.len + L::kTok - 1) / L::kTok;
 
-    // A2 = A log2(e); sums with A itself are formed with A2 and scaled back once
-    States<NS> A2, g, dA;               // g: a G of the token behind
-    A2.zero();
-    g.zero();
-    dA.zero();
-    if (at.live) {
-        A2.load_user(p.A + (int64_t)at.c * N, n0, N);
+    // A2 = A log2(e); the sum with A itself is formed with A2 and scaled back once
+    States<NS> A2[2], g[2], dA[2];      // g: a G of the token behind
+    load_rates<NS>(p, at, A2);
 #pragma unroll
-        for (int i = 0; i < P; ++i) A2.v[i] = mul2(A2.v[i], F2(1.44269504f));
-        if (!VARLEN && dfin != nullptr && at.seg == p.segs - 1) g.load_user(dfin + (at.b * p.channels + at.c) * N, n0, N);
-        for (int j = p.segs - 1; j > at.seg; --j) {
-            const int64_t k = seg_at<NS>(p, at.b, j, at.c);
-            const float sd = seg_d[k];
-            States<NS> own;
-            own.load(seg_g + k * L::kNP + n0);
-#pragma unroll
-            for (int i = 0; i < P; ++i) g.v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2.v[i])), g.v[i], own.v[i]);
-        }
+    for (int ch = 0; ch < 2; ++ch) {
+        g[ch].zero();
+        dA[ch].zero();
+        if (!VARLEN && dfin != nullptr && at.live[ch] && at.seg == p.segs - 1)
+            g[ch].load_user(dfin + (at.b * p.channels + at.c + ch) * N, n0, N);
     }
+    for (int j = p.segs - 1; j > at.seg; --j) add_segment<NS>(p, at, j, seg_g, seg_d, A2, g);
     const int row = at.row(), c = at.c0 + at.col();
-    if (row == 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            sm.D[at.slot(i)] = p.D != nullptr && c + i < at.cend ? p.D[c + i] : 0.f;
-            sm.bias[at.slot(i)] = p.bias != nullptr && c + i < at.cend ? p.bias[c + i] : 0.f;
-        }
-    }
+    load_per_channel<NS>(p, at, p.D, sm.D);
+    load_per_channel<NS>(p, at, p.bias, sm.bias);
 #pragma unroll
     for (int i = 0; i < V; ++i) sm.dD[i][threadIdx.x] = sm.db[i][threadIdx.x] = 0.f;
 
@@ -640,9 +666,12 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         const int64_t t = tb + row;
         bool ok = t < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
-        States<NS> h;
-        h.zero();
-        if (at.live) h.load(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c) * L::kNP + n0));
+        States<NS> h[2];
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+            h[ch].zero();
+            if (at.live[ch]) h[ch].load(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0));
+        }
         {
             BwdShare<T, NS> in;
             if (ok) in.load(p, at, x, dt, z, dy, t);
@@ -652,114 +681,137 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             bc.load(Cm, p.cs, p, at, tb, t1);
             bc.template put<VARLEN>(sm.C, sm.marks);
 #pragma unroll
-            for (int i = 0; i < V; i += 2) {
-                const int s = at.slot(i), s1 = at.slot(i + 1);
-                F2 d(0.f), u(0.f);
+            for (int i = 0; i < V / 2; ++i) {
+                const int s = at.slot_of(i);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                float2 e = make_float2(0.f, 0.f);
                 if (ok) {
-                    d = step2(p, in.dt.get(i) + sm.bias[s], in.dt.get(i + 1) + sm.bias[s1]);
-                    u = mul2(d, F2(in.x.get(i), in.x.get(i + 1)));
+                    const float2 bias = sm.bias[s];
+                    const F2 d = step2(p, in.dt.get(2 * i) + bias.x, in.dt.get(2 * i + 1) + bias.y);
+                    const F2 u = mul2(d, F2(in.x.get(2 * i), in.x.get(2 * i + 1)));
+                    v = make_float4(d.x(), u.x(), d.y(), u.y());
+                    e = make_float2(in.e(2 * i, z != nullptr), in.e(2 * i + 1, z != nullptr));
                 }
-                sm.dx[row][s] = make_float4(d.x(), d.x(), u.x(), u.x());
-                sm.dx[row][s1] = make_float4(d.y(), d.y(), u.y(), u.y());
-                sm.e[row][s] = ok ? in.e(i, z != nullptr) : 0.f;
-                sm.e[row][s1] = ok ? in.e(i + 1, z != nullptr) : 0.f;
+                sm.dx[row][s] = v;
+                sm.e[row][s] = e;
             }
         }
         __syncthreads();
 
 #pragma unroll 1
         for (int sub = 0; sub < BwdSmem<NS>::kSubs; ++sub) {
-            h.store(sm.start[sub][threadIdx.x]);
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) h[ch].store(sm.start[sub][ch][threadIdx.x]);
             if (sub == BwdSmem<NS>::kSubs - 1) break;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
-                F2 d2, dx2;
-                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
+                const float4 v = sm.dx[tt][at.slot];
                 States<NS> Bv;
                 Bv.load(sm.B + tt * L::kNP + n0);
-                h = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, h);
 #pragma unroll
-                for (int i = 0; i < P; ++i) h.v[i] = fma2(decay2(mul2(d2, A2.v[i])), h.v[i], mul2(dx2, Bv.v[i]));
+                for (int ch = 0; ch < 2; ++ch) {
+                    const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y);
+                    h[ch] = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, h[ch], ch);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) h[ch].v[i] = fma2(decay2(mul2(d2, A2[ch].v[i])), h[ch].v[i], mul2(dx2, Bv.v[i]));
+                }
             }
         }
 #pragma unroll 1
         for (int sub = BwdSmem<NS>::kSubs - 1; sub >= 0; --sub) {
-            States<NS> a[K], hs[K + 1];
-            hs[0].load(sm.start[sub][threadIdx.x]);
-            float ys[K], gb[K], ra[K];
+            States<NS> a[2][K], hs[2][K + 1];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int tt = sub * K + k;
-                F2 d2, dx2;
-                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
-                States<NS> Bv, Cv;
-                Bv.load(sm.B + tt * L::kNP + n0);
-                Cv.load(sm.C + tt * L::kNP + n0);
-                const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k]);
-                F2 s2(0.f);
+            for (int ch = 0; ch < 2; ++ch) hs[ch][0].load(sm.start[sub][ch][threadIdx.x]);
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    a[k].v[i] = decay2(mul2(d2, A2.v[i]));
-                    hs[k + 1].v[i] = fma2(a[k].v[i], hp.v[i], mul2(dx2, Bv.v[i]));
-                    s2 = fma2(Cv.v[i], hs[k + 1].v[i], s2);
-                }
-                ys[k] = s2.x() + s2.y();
-            }
+            for (int k0 = 0; k0 < K; k0 += 4) {
+                float ys[2][4];
 #pragma unroll
-            for (int k = K - 1; k >= 0; --k) {
-                const int tt = sub * K + k;
-                F2 d2, dx2;
-                load_pairs(&sm.dx[tt][at.pos], d2, dx2);
-                const F2 e2(sm.e[tt][at.pos]);
-                States<NS> Bv, Cv;
-                Bv.load(sm.B + tt * L::kNP + n0);
-                Cv.load(sm.C + tt * L::kNP + n0);
-                if (VARLEN && dfin != nullptr) {
-                    const int l = sm.marks.last[tt];
-                    if (l >= 0 && at.live) g.load_user(dfin + ((int64_t)l * p.channels + at.c) * N, n0, N);
-                }
-                const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[k]);
-                float bc[2 * NS];
-                F2 gb2(0.f), ra2(0.f);
+                for (int k = k0; k < k0 + 4; ++k) {
+                    const int tt = sub * K + k;
+                    const float4 v = sm.dx[tt][at.slot];
+                    States<NS> Bv, Cv;
+                    Bv.load(sm.B + tt * L::kNP + n0);
+                    Cv.load(sm.C + tt * L::kNP + n0);
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const F2 G = fma2(e2, Cv.v[i], g.v[i]);
-                    mul2(dx2, G).get(bc[2 * i], bc[2 * i + 1]);
-                    mul2(e2, hs[k + 1].v[i]).get(bc[NS + 2 * i], bc[NS + 2 * i + 1]);
-                    gb2 = fma2(G, Bv.v[i], gb2);
-                    g.v[i] = mul2(a[k].v[i], G);
-                    const F2 r = mul2(g.v[i], hp.v[i]);
-                    ra2 = fma2(r, A2.v[i], ra2);
-                    dA.v[i] = fma2(d2, r, dA.v[i]);
-                }
-                gb[k] = gb2.x() + gb2.y();
-                ra[k] = ra2.x() + ra2.y();
-                if (VARLEN) {
-                    const int f = sm.marks.first[tt];
-                    if (f >= 0) {
-                        if (dinit != nullptr && at.live) g.store_user(dinit + ((int64_t)f * p.channels + at.c) * N, n0, N);
-                        g.zero();
+                    for (int ch = 0; ch < 2; ++ch) {
+                        const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y);
+                        const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[ch][k], ch);
+                        F2 s2(0.f);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            a[ch][k].v[i] = decay2(mul2(d2, A2[ch].v[i]));
+                            hs[ch][k + 1].v[i] = fma2(a[ch][k].v[i], hp.v[i], mul2(dx2, Bv.v[i]));
+                            s2 = i == 0 ? mul2(Cv.v[i], hs[ch][k + 1].v[i]) : fma2(Cv.v[i], hs[ch][k + 1].v[i], s2);
+                        }
+                        ys[ch][k - k0] = s2.x() + s2.y();
                     }
                 }
-                const int first = sum8<2 * NS>(bc, at.lane);
-                constexpr int LEFT = 2 * NS >= 8 ? 2 * NS / 8 : 1;
-#pragma unroll
-                for (int i = 0; i < LEFT; ++i) {
-                    const int w = first + i;            // dB of state n0 + w, or dC of state n0 + w - NS
-                    sm.dbc[at.warp][tt][(w < NS ? n0 + w : L::kNP + n0 + w - NS)] = bc[i];
-                }
+                const float y0 = sum4(ys[0], at.q), y1 = sum4(ys[1], at.q);
+                sm.y[sub * K + k0 + at.q][at.slot] = make_float2(y0, y1);
             }
-            __syncwarp();               // the four lanes of a channel are done with its (d, d x) of this sub-tile
 #pragma unroll
-            for (int k = 0; k < K; k += 4) {
-                const int tt = sub * K + k + at.q;
-                const float y4[4] = {ys[k], ys[k + 1], ys[k + 2], ys[k + 3]}, g4[4] = {gb[k], gb[k + 1], gb[k + 2], gb[k + 3]},
-                            r4[4] = {ra[k], ra[k + 1], ra[k + 2], ra[k + 3]};
-                const float sy = sum4(y4, at.q), sg = sum4(g4, at.q), sr = sum4(r4, at.q);
-                float4& o = sm.dx[tt][at.pos];
-                o.y = sy;
-                *reinterpret_cast<float2*>(&o.z) = make_float2(sg, sr * 0.69314718f);
+            for (int k0 = K - 4; k0 >= 0; k0 -= 4) {
+                float gb[2][4], ra[2][4];
+#pragma unroll
+                for (int k = k0 + 3; k >= k0; --k) {
+                    const int tt = sub * K + k;
+                    const float4 v = sm.dx[tt][at.slot];
+                    const float2 e = sm.e[tt][at.slot];
+                    States<NS> Bv, Cv;
+                    Bv.load(sm.B + tt * L::kNP + n0);
+                    Cv.load(sm.C + tt * L::kNP + n0);
+                    F2 dB[P], dC[P];
+#pragma unroll
+                    for (int ch = 0; ch < 2; ++ch) {
+                        const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y), e2(ch ? e.y : e.x);
+                        if (VARLEN && dfin != nullptr) {
+                            const int l = sm.marks.last[tt];
+                            if (l >= 0 && at.live[ch]) g[ch].load_user(dfin + ((int64_t)l * p.channels + at.c + ch) * N, n0, N);
+                        }
+                        const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[ch][k], ch);
+                        F2 gb2(0.f), ra2(0.f);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            const F2 G = fma2(e2, Cv.v[i], g[ch].v[i]);
+                            dB[i] = ch == 0 ? mul2(dx2, G) : fma2(dx2, G, dB[i]);
+                            dC[i] = ch == 0 ? mul2(e2, hs[ch][k + 1].v[i]) : fma2(e2, hs[ch][k + 1].v[i], dC[i]);
+                            gb2 = i == 0 ? mul2(G, Bv.v[i]) : fma2(G, Bv.v[i], gb2);
+                            g[ch].v[i] = mul2(a[ch][k].v[i], G);
+                            const F2 r = mul2(g[ch].v[i], hp.v[i]);
+                            ra2 = i == 0 ? mul2(r, A2[ch].v[i]) : fma2(r, A2[ch].v[i], ra2);
+                            dA[ch].v[i] = fma2(d2, r, dA[ch].v[i]);
+                        }
+                        gb[ch][k - k0] = gb2.x() + gb2.y();
+                        ra[ch][k - k0] = ra2.x() + ra2.y();
+                        if (VARLEN) {
+                            const int f = sm.marks.first[tt];
+                            if (f >= 0) {
+                                if (dinit != nullptr && at.live[ch]) g[ch].store_user(dinit + ((int64_t)f * p.channels + at.c + ch) * N, n0, N);
+                                g[ch].zero();
+                            }
+                        }
+                    }
+                    float bc[2 * NS];
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        dB[i].get(bc[2 * i], bc[2 * i + 1]);
+                        dC[i].get(bc[NS + 2 * i], bc[NS + 2 * i + 1]);
+                    }
+                    const int first = sum8<2 * NS>(bc, at.lane);
+                    constexpr int LEFT = 2 * NS >= 8 ? 2 * NS / 8 : 1;
+#pragma unroll
+                    for (int i = 0; i < LEFT; ++i) {
+                        const int w = first + i;            // dB of state n0 + w, or dC of state n0 + w - NS
+                        sm.dbc[at.warp][tt][(w < NS ? n0 + w : L::kNP + n0 + w - NS)] = bc[i];
+                    }
+                }
+                const float g0 = sum4(gb[0], at.q), g1 = sum4(gb[1], at.q), r0 = sum4(ra[0], at.q), r1 = sum4(ra[1], at.q);
+                __syncwarp();               // the four lanes of a channel are done with its d x and e of these tokens
+                const int tt = sub * K + k0 + at.q;
+                sm.dx[tt][at.slot].y = g0;
+                sm.dx[tt][at.slot].w = g1;
+                sm.e[tt][at.slot] = make_float2(r0 * 0.69314718f, r1 * 0.69314718f);
             }
         }
         __syncthreads();
@@ -777,21 +829,20 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             float ox[V], od[V], oz[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int s = at.slot(i);
+                const int s = at.slot_of(i / 2);
                 ox[i] = od[i] = oz[i] = 0.f;
                 if (ok) {
-                    const float4 v = sm.dx[row][s];         // d, s, sum G B, sum A r
-                    const float xv = in.x.get(i), D = sm.D[s], e = sm.e[row][s];
-                    ox[i] = fmaf(v.x, v.z, D * e);
-                    od[i] = fmaf(xv, v.z, v.w);
-                    if (p.softplus) {
-                        const float raw = in.dt.get(i) + sm.bias[s];
-                        if (!(raw > 20.f)) od[i] *= fbla::seq::sigmoid<T>(raw);
-                    }
-                    if (z != nullptr) {
-                        const float zv = in.z.get(i), gate = fbla::seq::sigmoid<T>(zv);
-                        oz[i] = in.dy.get(i) * fmaf(D, xv, v.y) * gate * (1.f + zv * (1.f - gate));
-                    }
+                    const float4 v = sm.dx[row][s];         // d, sum G B of either channel
+                    const float2 r2 = sm.e[row][s], y2 = sm.y[row][s], D2 = sm.D[s], b2 = sm.bias[s];
+                    const float d = i & 1 ? v.z : v.x, gB = i & 1 ? v.w : v.y, rA = i & 1 ? r2.y : r2.x, sy = i & 1 ? y2.y : y2.x;
+                    const float D = i & 1 ? D2.y : D2.x, raw = in.dt.get(i) + (i & 1 ? b2.y : b2.x);
+                    const float xv = in.x.get(i), zv = in.z.get(i), g = in.dy.get(i);
+                    const float gate = z != nullptr ? fbla::seq::sigmoid<T>(zv) : 1.f;
+                    const float e = z != nullptr ? g * zv * gate : g;
+                    ox[i] = fmaf(d, gB, D * e);
+                    od[i] = fmaf(xv, gB, rA);
+                    if (p.softplus && !(raw > 20.f)) od[i] *= fbla::seq::sigmoid<T>(raw);
+                    if (z != nullptr) oz[i] = g * fmaf(D, xv, sy) * gate * (1.f + zv * (1.f - gate));
                     sm.dD[i][threadIdx.x] += e * xv;
                     sm.db[i][threadIdx.x] += od[i];
                 }
@@ -814,9 +865,12 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         part_D[bs * p.channels + at.c0 + threadIdx.x] = sD;
         part_bias[bs * p.channels + at.c0 + threadIdx.x] = sb;
     }
-    if (!at.live) return;
-    dA.store_user(part_A + (bs * p.channels + at.c) * N, n0, N);
-    if (!VARLEN && dinit != nullptr && at.seg == 0) g.store_user(dinit + (at.b * p.channels + at.c) * N, n0, N);
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        if (!at.live[ch]) continue;
+        dA[ch].store_user(part_A + (bs * p.channels + at.c + ch) * N, n0, N);
+        if (!VARLEN && dinit != nullptr && at.seg == 0) g[ch].store_user(dinit + (at.b * p.channels + at.c + ch) * N, n0, N);
+    }
 }
 
 // dB, dC (batch, token, group, N) from the channel tiles' sums, tiles in order.
@@ -833,24 +887,28 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const float* __restrict__ 
     (w < NP ? dB : dC)[r * N + n] = from_f<T>(s);
 }
 
-// One token per row, the state updated in place.
+// One token per row, the state updated in place.  Four lanes per channel: a state is read and written once, 16 bytes
+// per lane where N allows, and that traffic is what bounds it (8 N bytes per channel against 8 of everything else).
+constexpr int kStepChannels = 32;
 template <typename T, int NS>
-__global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
-                                                             const T* __restrict__ Bm, const T* __restrict__ Cm,
-                                                             const T* __restrict__ z, float* __restrict__ state, T* __restrict__ y) {
-    const Place<NS> at(p);
-    const int N = p.states, n0 = at.q * NS;
+__global__ void __launch_bounds__(4 * kStepChannels) scan_step_kernel(const ScanParams p, const T* __restrict__ x, const T* __restrict__ dt,
+                                                                      const T* __restrict__ Bm, const T* __restrict__ Cm,
+                                                                      const T* __restrict__ z, float* __restrict__ state, T* __restrict__ y) {
+    const int64_t b = blockIdx.y;
+    const int c = blockIdx.x * kStepChannels + threadIdx.x / 4, q = threadIdx.x & 3, N = p.states, n0 = q * NS;
+    const bool live = c < p.channels;
     float acc = 0.f, xv = 0.f;
-    if (at.live) {
-        float* hp = state + (at.b * p.channels + at.c) * N;
+    if (live) {
+        float* hp = state + (b * p.channels + c) * N;
+        const int group = c / (p.channels / p.groups);
         States<NS> h, A;
         h.load_user(hp, n0, N);
-        A.load_user(p.A + (int64_t)at.c * N, n0, N);
-        const T* Bp = Bm + at.b * p.bs[0] + at.group * p.bs[2];
-        const T* Cp = Cm + at.b * p.cs[0] + at.group * p.cs[2];
-        xv = to_f<T>(x[at.b * p.xs[0] + at.c]);
-        float d = to_f<T>(dt[at.b * p.ds[0] + at.c]);
-        if (p.bias != nullptr) d += p.bias[at.c];
+        A.load_user(p.A + (int64_t)c * N, n0, N);
+        const T* Bp = Bm + b * p.bs[0] + group * p.bs[2];
+        const T* Cp = Cm + b * p.cs[0] + group * p.cs[2];
+        xv = to_f<T>(x[b * p.xs[0] + c]);
+        float d = to_f<T>(dt[b * p.ds[0] + c]);
+        if (p.bias != nullptr) d += p.bias[c];
         if (p.softplus) d = fbla::seq::softplus(d);
         F2 s2(0.f);
 #pragma unroll
@@ -866,13 +924,13 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const ScanParams p,
     }
     acc += __shfl_xor_sync(0xffffffffu, acc, 1);
     acc += __shfl_xor_sync(0xffffffffu, acc, 2);
-    if (at.live && at.q == 0) {
-        if (p.D != nullptr) acc = fmaf(p.D[at.c], xv, acc);
+    if (live && q == 0) {
+        if (p.D != nullptr) acc = fmaf(p.D[c], xv, acc);
         if (z != nullptr) {
-            const float zv = to_f<T>(z[at.b * p.zs[0] + at.c]);
+            const float zv = to_f<T>(z[b * p.zs[0] + c]);
             acc *= zv * fbla::seq::sigmoid<T>(zv);
         }
-        y[at.b * p.channels + at.c] = from_f<T>(acc);
+        y[b * p.channels + c] = from_f<T>(acc);
     }
 }
 
@@ -936,9 +994,9 @@ int resolve(const fbla_scan_problem* p, ScanParams* r) {
     return FBLA_OK;
 }
 
-// Packs of 8 (4 for states above 16) elements: every row and every CTA's first channel on a boundary.
+// Packs of a multiple of 8 elements: every row and every CTA's first channel on a boundary.
 bool can_vec(const ScanParams& p, int elem, bool z, bool dy, std::initializer_list<const void*> ptrs) {
-    const int v = tok_of(p.states) == 16 ? 4 : 8;
+    const int v = 8;        // 16 bytes of the 16-bit types; an fp32 pack is two accesses
     const int64_t bytes = v * elem > 16 ? 16 : v * elem;
     bool ok = (p.channels / p.groups) % v == 0 && p.xs[0] % v == 0 && p.xs[1] % v == 0 && p.ds[0] % v == 0 && p.ds[1] % v == 0;
     if (z) ok = ok && p.zs[0] % v == 0 && p.zs[1] % v == 0;
@@ -1043,7 +1101,8 @@ template <typename T, int NS, bool VARLEN> cudaError_t run_bwd(const ScanParams&
 }
 
 template <typename T, int NS> cudaError_t run_step(const ScanParams& p, const ScanTensors& a, cudaStream_t st) {
-    scan_step_kernel<T, NS><<<scan_grid(p), kThreads, 0, st>>>(p, (const T*)a.x, (const T*)a.dt, (const T*)a.B, (const T*)a.C, (const T*)a.z,
+    const dim3 grid((unsigned)((p.channels + kStepChannels - 1) / kStepChannels), (unsigned)p.batch);
+    scan_step_kernel<T, NS><<<grid, 4 * kStepChannels, 0, st>>>(p, (const T*)a.x, (const T*)a.dt, (const T*)a.B, (const T*)a.C, (const T*)a.z,
                                                                a.fin, (T*)a.y);
     fbla::note_launches(1);
     return cudaGetLastError();
