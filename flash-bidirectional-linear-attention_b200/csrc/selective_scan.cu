@@ -482,9 +482,19 @@ template <typename T, int NS> struct BwdShare {
         load_row<T, V>(dyp + at.b * p.gs[0] + t * p.gs[1], c, at.cend, p.vec, dy);
         if (zp != nullptr) load_row<T, V>(zp + at.b * p.zs[0] + t * p.zs[1], c, at.cend, p.vec, z);
     }
+    // e = dy silu(z)
     __device__ __forceinline__ float e(int i, bool gated) const {
         const float g = dy.get(i);
         return gated ? g * z.get(i) * fbla::seq::sigmoid<T>(z.get(i)) : g;
+    }
+    // and dy silu'(z), what dz is of the ungated output
+    __device__ __forceinline__ float e(int i, bool gated, float& slope) const {
+        const float g = dy.get(i);
+        slope = 0.f;
+        if (!gated) return g;
+        const float zv = z.get(i), gate = fbla::seq::sigmoid<T>(zv), gg = g * gate;
+        slope = gg * fmaf(zv, 1.f - gate, 1.f);
+        return gg * zv;
     }
 };
 
@@ -608,13 +618,15 @@ template <int M> __device__ __forceinline__ int sum8(float (&v)[M], int lane) {
 template <int NS> struct BwdSmem {
     using L = Tile<NS>;
     static constexpr int kSubs = L::kTok / L::kSub;
-    float4 dx[L::kTok][kRow4];                      // per two channels (d, d x, d, d x); behind its reverse pass sum G B for d x
-    float2 e[L::kTok][kRow2];                       // e; behind the reverse pass sum A r
+    float4 dx[L::kTok][kRow4];                      // per two channels (d, d x, d, d x); behind its reverse pass sum A r for d x
+    float2 e[L::kTok][kRow2];                       // dy silu(z)
+    float2 slope[L::kTok][kRow2];                   // dy silu'(z)
     float2 y[L::kTok][kRow2];                       // s = sum C h
+    float2 gB[L::kTok][kRow2];                      // sum G B
     float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
     float start[kSubs][2][kThreads][NS];            // each thread's states at the starts of the sub-tiles
     float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its channels
-    float dD[L::kVPT][kThreads], db[L::kVPT][kThreads];
+    float4 acc[L::kVPT / 2][kThreads];              // each thread's sums for dD (two channels) and dbias
     float2 D[kCB / 2], bias[kCB / 2];
     Marks marks;
 };
@@ -655,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     load_per_channel<NS>(p, at, p.D, sm.D);
     load_per_channel<NS>(p, at, p.bias, sm.bias);
 #pragma unroll
-    for (int i = 0; i < V; ++i) sm.dD[i][threadIdx.x] = sm.db[i][threadIdx.x] = 0.f;
+    for (int i = 0; i < V / 2; ++i) sm.acc[i][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
 
     for (int64_t tb = t0 + (t1 - 1 - t0) / L::kTok * L::kTok; tb >= t0; tb -= L::kTok) {
         __syncthreads();
@@ -684,16 +696,21 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             for (int i = 0; i < V / 2; ++i) {
                 const int s = at.slot_of(i);
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                float2 e = make_float2(0.f, 0.f);
+                float2 e = make_float2(0.f, 0.f), slope = e;
                 if (ok) {
                     const float2 bias = sm.bias[s];
+                    const float x0 = in.x.get(2 * i), x1 = in.x.get(2 * i + 1);
                     const F2 d = step2(p, in.dt.get(2 * i) + bias.x, in.dt.get(2 * i + 1) + bias.y);
-                    const F2 u = mul2(d, F2(in.x.get(2 * i), in.x.get(2 * i + 1)));
+                    const F2 u = mul2(d, F2(x0, x1));
                     v = make_float4(d.x(), u.x(), d.y(), u.y());
-                    e = make_float2(in.e(2 * i, z != nullptr), in.e(2 * i + 1, z != nullptr));
+                    e.x = in.e(2 * i, z != nullptr, slope.x);
+                    e.y = in.e(2 * i + 1, z != nullptr, slope.y);
+                    float2& sum = *reinterpret_cast<float2*>(&sm.acc[i][threadIdx.x].x);
+                    sum = make_float2(fmaf(e.x, x0, sum.x), fmaf(e.y, x1, sum.y));
                 }
                 sm.dx[row][s] = v;
                 sm.e[row][s] = e;
+                if (z != nullptr) sm.slope[row][s] = slope;
             }
         }
         __syncthreads();
@@ -807,11 +824,11 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                     }
                 }
                 const float g0 = sum4(gb[0], at.q), g1 = sum4(gb[1], at.q), r0 = sum4(ra[0], at.q), r1 = sum4(ra[1], at.q);
-                __syncwarp();               // the four lanes of a channel are done with its d x and e of these tokens
+                __syncwarp();               // the four lanes of a channel are done with its d x of these tokens
                 const int tt = sub * K + k0 + at.q;
-                sm.dx[tt][at.slot].y = g0;
-                sm.dx[tt][at.slot].w = g1;
-                sm.e[tt][at.slot] = make_float2(r0 * 0.69314718f, r1 * 0.69314718f);
+                sm.gB[tt][at.slot] = make_float2(g0, g1);
+                sm.dx[tt][at.slot].y = r0 * 0.69314718f;
+                sm.dx[tt][at.slot].w = r1 * 0.69314718f;
             }
         }
         __syncthreads();
@@ -824,28 +841,37 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             part_bc[((((int64_t)at.tile_in_group * p.batch + at.b) * p.len + tb + tt) * p.groups + at.group) * (2 * L::kNP) + w] = s;
         }
         if (t < t1) {
-            BwdShare<T, NS> in;
-            if (ok) in.load(p, at, x, dt, z, dy, t);
+            Pack<T, V> xv, dtv;
+            xv.zero();
+            dtv.zero();
+            if (ok) {
+                load_row<T, V>(x + at.b * p.xs[0] + t * p.xs[1], c, at.cend, p.vec, xv);
+                load_row<T, V>(dt + at.b * p.ds[0] + t * p.ds[1], c, at.cend, p.vec, dtv);
+            }
             float ox[V], od[V], oz[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < V; i += 2) {
                 const int s = at.slot_of(i / 2);
-                ox[i] = od[i] = oz[i] = 0.f;
-                if (ok) {
-                    const float4 v = sm.dx[row][s];         // d, sum G B of either channel
-                    const float2 r2 = sm.e[row][s], y2 = sm.y[row][s], D2 = sm.D[s], b2 = sm.bias[s];
-                    const float d = i & 1 ? v.z : v.x, gB = i & 1 ? v.w : v.y, rA = i & 1 ? r2.y : r2.x, sy = i & 1 ? y2.y : y2.x;
-                    const float D = i & 1 ? D2.y : D2.x, raw = in.dt.get(i) + (i & 1 ? b2.y : b2.x);
-                    const float xv = in.x.get(i), zv = in.z.get(i), g = in.dy.get(i);
-                    const float gate = z != nullptr ? fbla::seq::sigmoid<T>(zv) : 1.f;
-                    const float e = z != nullptr ? g * zv * gate : g;
-                    ox[i] = fmaf(d, gB, D * e);
-                    od[i] = fmaf(xv, gB, rA);
-                    if (p.softplus && !(raw > 20.f)) od[i] *= fbla::seq::sigmoid<T>(raw);
-                    if (z != nullptr) oz[i] = g * fmaf(D, xv, sy) * gate * (1.f + zv * (1.f - gate));
-                    sm.dD[i][threadIdx.x] += e * xv;
-                    sm.db[i][threadIdx.x] += od[i];
+                const float4 v = sm.dx[row][s];             // d, sum A r
+                const float2 e = sm.e[row][s], gB = sm.gB[row][s], D = sm.D[s], bias = sm.bias[s];
+                const float x0 = xv.get(i), x1 = xv.get(i + 1);
+                ox[i] = fmaf(v.x, gB.x, D.x * e.x);
+                ox[i + 1] = fmaf(v.z, gB.y, D.y * e.y);
+                od[i] = fmaf(x0, gB.x, v.y);
+                od[i + 1] = fmaf(x1, gB.y, v.w);
+                if (p.softplus) {
+                    const float r0 = dtv.get(i) + bias.x, r1 = dtv.get(i + 1) + bias.y;
+                    od[i] *= r0 > 20.f ? 1.f : fbla::seq::sigmoid<T>(r0);
+                    od[i + 1] *= r1 > 20.f ? 1.f : fbla::seq::sigmoid<T>(r1);
                 }
+                if (z != nullptr) {
+                    const float2 slope = sm.slope[row][s], y2 = sm.y[row][s];
+                    oz[i] = slope.x * fmaf(D.x, x0, y2.x);
+                    oz[i + 1] = slope.y * fmaf(D.y, x1, y2.y);
+                }
+                if (!ok) ox[i] = ox[i + 1] = od[i] = od[i + 1] = oz[i] = oz[i + 1] = 0.f;
+                float2& sum = *reinterpret_cast<float2*>(&sm.acc[i / 2][threadIdx.x].z);
+                sum = make_float2(sum.x + od[i], sum.y + od[i + 1]);
             }
             const int64_t o = (at.b * p.len + t) * p.channels;
             store_row<T, V>(dx + o, c, at.cend, p.vec, ox);
@@ -859,8 +885,9 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         const int k = threadIdx.x / V, i = threadIdx.x % V;
         float sD = 0.f, sb = 0.f;
         for (int r = 0; r < L::kTok; ++r) {
-            sD += sm.dD[i][r * L::kTPR + k];
-            sb += sm.db[i][r * L::kTPR + k];
+            const float4 v = sm.acc[i / 2][r * L::kTPR + k];
+            sD += i & 1 ? v.y : v.x;
+            sb += i & 1 ? v.w : v.z;
         }
         part_D[bs * p.channels + at.c0 + threadIdx.x] = sD;
         part_bias[bs * p.channels + at.c0 + threadIdx.x] = sb;

@@ -78,9 +78,6 @@ __device__ __forceinline__ float exp_full(float x) {
 // A NaN goes through fminf / fmaxf as the other operand: keep it.
 __device__ __forceinline__ float exp_of(float x) { return x != x ? x : exp_full(x); }
 
-// 1 / (1 + e^-x); for 16-bit results the approximate exponential (2^-22 relative) is far below the rounding.
-template <typename T> __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-template <> __device__ __forceinline__ float sigmoid<float>(float x) { return __frcp_rn(1.f + exp_of(-x)); }
 
 // Two fp32 values in one 64-bit register: one instruction for two multiply-adds.  The rate of the multiply-add
 // units is the same (128 per clock and SM measured either way), half of the issue slots are left to others.
@@ -114,6 +111,11 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+
+// 1 / (1 + e^-x); for 16-bit results the special functions' errors (2^-21 with that of the product for |x| < 16)
+// are far below the rounding.
+template <typename T> __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(x * -1.44269504f)); }
+template <> __device__ __forceinline__ float sigmoid<float>(float x) { return __frcp_rn(1.f + exp_of(-x)); }
 
 // log(1 + e^v) of two values: max(v, 0) + log1p(w) with w = e^-|v| in (0, 1], and log1p(w) = 2 atanh(w / (2 + w))
 // as its series in s = w / (2 + w) <= 1/3 (the first term left out is s^14 / 15 = 1.4e-8 relative).  e^-|v| is the
