@@ -11,7 +11,8 @@
 // inputs (and, backward, the last W-1 gradients) in registers: x is read once, plus W-1 tokens per run.
 // Tokens go by in groups of four, and the next group's loads are on their way while one is worked on: with
 // one load in flight per thread a B8-T4096-C2048 forward took 124 us and the backward 298.
-// The weight gradient is summed in registers over a thread's run, in shared memory over the runs of a
+// Two channels share the packed fp32 instructions: in plain ones the arithmetic (W products per element forward,
+// 3 W + 1 backward, a sigmoid) takes as long as the memory.  The weight gradient is summed in registers over a thread's run, in shared memory over the runs of a
 // block, and then over the blocks by a kernel of its own: no atomics, the same bits on every run.
 #include <type_traits>
 
@@ -49,6 +50,9 @@ namespace {
 
 using fbla::from_f;
 using fbla::to_f;
+using fbla::seq::F2;
+using fbla::seq::fma2;
+using fbla::seq::mul2;
 using fbla::seq::Pack;
 using fbla::seq::seq_of;
 using fbla::seq::SeqSpan;
@@ -62,10 +66,6 @@ struct ConvParams {
     const void *w, *bias;       // w (channels, W), bias (channels) or NULL; fp32 when w32, else the type of x
 };
 
-template <typename T> __device__ __forceinline__ float param(const ConvParams& p, const void* base, int64_t i) {
-    return p.w32 ? reinterpret_cast<const float*>(base)[i] : to_f<T>(reinterpret_cast<const T*>(base)[i]);
-}
-
 __device__ __forceinline__ SeqSpan span_of(const ConvParams& p, int64_t b, int64_t t) {
     if (p.cu != nullptr) return seq_of(p.cu, p.num_seqs, t);
     SeqSpan s;
@@ -75,10 +75,30 @@ __device__ __forceinline__ SeqSpan span_of(const ConvParams& p, int64_t b, int64
     return s;
 }
 
+// V channels as pairs; with one channel the second half of the pair is idle
+template <int V> struct Lanes {
+    static constexpr int P = (V + 1) / 2;
+    F2 v[P];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = F2(0.f);
+    }
+    template <typename T> __device__ __forceinline__ void from(const Pack<T, V>& p) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = F2(p.get(2 * i), 2 * i + 1 < V ? p.get(2 * i + 1 < V ? 2 * i + 1 : 0) : 0.f);
+    }
+    template <typename T> __device__ __forceinline__ void to(Pack<T, V>& p) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            p.set(2 * i, v[i].x());
+            if (2 * i + 1 < V) p.set(2 * i + 1 < V ? 2 * i + 1 : 0, v[i].y());
+        }
+    }
+};
+
 // Input of token u (which may lie before its sequence: initial state, or zero), V channels from c.
 template <typename T, int W, int V>
-__device__ __forceinline__ void input_of(const ConvParams& p, const T* x, const T* init, const SeqSpan& s, int64_t b, int64_t u,
-                                         int c, float (&out)[V]) {
+__device__ __forceinline__ Lanes<V> input_of(const ConvParams& p, const T* x, const T* init, const SeqSpan& s, int64_t b, int64_t u, int c) {
     Pack<T, V> v;
     if (u >= s.lo && s.s >= 0) {
         v.load(x + b * p.xs[0] + u * p.xs[1] + c);
@@ -87,19 +107,21 @@ __device__ __forceinline__ void input_of(const ConvParams& p, const T* x, const 
     } else {
         v.zero();
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = v.get(i);
+    Lanes<V> r;
+    r.from(v);
+    return r;
 }
 
-template <typename T> __device__ __forceinline__ float activate(float x, int silu) {
-    return silu ? x * fbla::seq::sigmoid<T>(x) : x;
+template <typename T> __device__ __forceinline__ F2 sigmoid2(F2 x) {
+    return F2(fbla::seq::sigmoid<T>(x.x()), fbla::seq::sigmoid<T>(x.y()));
 }
+template <typename T, bool SILU> __device__ __forceinline__ F2 activate(F2 x) { return SILU ? mul2(x, sigmoid2<T>(x)) : x; }
 
-// dy times the slope of the activation at p
-template <typename T> __device__ __forceinline__ float pre_grad(float dy, float x, int silu) {
-    if (!silu) return dy;
-    const float sg = fbla::seq::sigmoid<T>(x);
-    return dy * sg * fmaf(x, 1.f - sg, 1.f);
+// dy times the slope of the activation at x: silu'(x) = s (1 + x (1 - s)), s = sigmoid(x)
+template <typename T, bool SILU> __device__ __forceinline__ F2 pre_grad(F2 dy, F2 x) {
+    if (!SILU) return dy;
+    const F2 s = sigmoid2<T>(x);
+    return mul2(mul2(dy, s), fma2(x, fma2(s, F2(-1.f), F2(1.f)), F2(1.f)));
 }
 
 constexpr int U = 4;            // tokens of a group
@@ -111,22 +133,34 @@ template <typename T, int V> __device__ __forceinline__ void load_group(const T*
 }
 
 // Parameters of V channels
-template <typename T, int W, int V> struct Filter {
-    float w[W][V], bias[V];
-    __device__ __forceinline__ void load(const ConvParams& p, int c) {
+template <int W, int V> struct Filter {
+    Lanes<V> w[W], bias;
+    template <typename WT> __device__ __forceinline__ void load_as(const WT* wp, const WT* bp, int c) {
+        Pack<WT, V> k[W], b;                // (V, W) consecutive elements
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            bias[i] = p.bias != nullptr ? param<T>(p, p.bias, c + i) : 0.f;
+        for (int j = 0; j < W; ++j) k[j].load(wp + (int64_t)c * W + j * V);
+        if (bp != nullptr) b.load(bp + c);
+        else b.zero();
+        bias.from(b);
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[j][i] = param<T>(p, p.w, (int64_t)(c + i) * W + j);
+        for (int j = 0; j < W; ++j) {
+            Pack<WT, V> t;
+#pragma unroll
+            for (int i = 0; i < V; ++i) t.e[i] = k[(i * W + j) / V].e[(i * W + j) % V];
+            w[j].from(t);
         }
+    }
+    template <typename T> __device__ __forceinline__ void load(const ConvParams& p, int c) {
+        if (p.w32) load_as((const float*)p.w, (const float*)p.bias, c);
+        else load_as((const T*)p.w, (const T*)p.bias, c);
     }
 };
 
 // A thread walks over its run piece by piece, a piece being the run's tokens of one sequence.
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(256) conv_fwd_kernel(const ConvParams p, const T* __restrict__ x, const T* __restrict__ init,
-                                                       T* __restrict__ y) {
+template <typename T, int W, int V, bool SILU>
+__global__ void __launch_bounds__(256, 2) conv_fwd_kernel(const ConvParams p, const T* __restrict__ x, const T* __restrict__ init,
+                                                          T* __restrict__ y) {
+    constexpr int P = Lanes<V>::P;
     const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
     const int64_t b = blockIdx.z;
     const int64_t t0 = ((int64_t)blockIdx.y * blockDim.y + threadIdx.y) * p.run;
@@ -134,8 +168,8 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(const ConvParams p, const
     const int64_t t1 = min(p.len, t0 + p.run);
     const T* xb = x + b * p.xs[0] + c;
     T* yb = y + b * p.len * p.channels + c;
-    Filter<T, W, V> f;
-    f.load(p, c);
+    Filter<W, V> f;
+    f.template load<T>(p, c);
     for (int64_t a = t0; a < t1;) {
         const SeqSpan s = span_of(p, b, a);
         const int64_t end = min(t1, s.hi);
@@ -147,31 +181,27 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(const ConvParams p, const
         }
         Pack<T, V> next[U];
         load_group<T, V>(xb, p.xs[1], a, end, next);
-        float in[W - 1 + U][V];         // the last W-1 inputs, then the group's
+        Lanes<V> in[W - 1 + U];         // the last W-1 inputs, then the group's
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c, in[j]);
+        for (int j = 0; j < W - 1; ++j) in[j] = input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c);
         for (; a < end; a += U) {
 #pragma unroll
-            for (int k = 0; k < U; ++k)
-#pragma unroll
-                for (int i = 0; i < V; ++i) in[W - 1 + k][i] = next[k].get(i);
-            load_group<T, V>(xb, p.xs[1], a + U, end, next);
-#pragma unroll
             for (int k = 0; k < U; ++k) {
-                Pack<T, V> out;
+                in[W - 1 + k].from(next[k]);
+                if (a + U + k < end) next[k].load(xb + (a + U + k) * p.xs[1]);
+                Lanes<V> o = f.bias;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float o = f.bias[i];
+                for (int i = 0; i < P; ++i) {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) o = fmaf(f.w[j][i], in[k + j][i], o);
-                    out.set(i, activate<T>(o, p.silu));
+                    for (int j = 0; j < W; ++j) o.v[i] = fma2(f.w[j].v[i], in[k + j].v[i], o.v[i]);
+                    o.v[i] = activate<T, SILU>(o.v[i]);
                 }
+                Pack<T, V> out;
+                o.to(out);
                 if (a + k < end) out.store(yb + (a + k) * p.channels);
             }
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) in[j][i] = in[j + U][i];
+            for (int j = 0; j < W - 1; ++j) in[j] = in[j + U];
         }
         a = end;
     }
@@ -197,103 +227,102 @@ __global__ void __launch_bounds__(256) conv_final_kernel(const ConvParams p, con
 // dx, and per block the sums for dw and dbias (part: [block of tokens][W + 1][channels]).
 // The gradient g of a token reaches back to the W-1 inputs before it, so a piece is walked W-1 tokens beyond its
 // end: those belong to the next run, or are zero where the sequence ends; only their g is needed here.
-template <typename T, int W, int V>
+template <typename T, int W, int V, bool SILU>
 __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, const T* __restrict__ x, const T* __restrict__ init,
                                                           const T* __restrict__ dy, const T* __restrict__ dfin, T* __restrict__ dx,
                                                           float* __restrict__ part) {
+    constexpr int P = Lanes<V>::P;
     extern __shared__ float red[];              // [blockDim.y][W + 1][blockDim.x * V]
     const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
     const int64_t b = blockIdx.z;
     const int64_t t0 = ((int64_t)blockIdx.y * blockDim.y + threadIdx.y) * p.run;
-    float dw[W][V], db[V];
+    Lanes<V> dw[W], db;
+    db.zero();
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        db[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][i] = 0.f;
-    }
+    for (int j = 0; j < W; ++j) dw[j].zero();
     if (c < p.channels && t0 < p.len) {
         const int64_t t1 = min(p.len, t0 + p.run);
         const T* xb = x + b * p.xs[0] + c;
         const T* gb = dy + b * p.gs[0] + c;
-        T* db_out = dx + b * p.len * p.channels + c;
-        Filter<T, W, V> f;
-        f.load(p, c);
+        T* ob = dx + b * p.len * p.channels + c;
+        Filter<W, V> f;
+        f.template load<T>(p, c);
         for (int64_t a = t0; a < t1;) {
             const SeqSpan s = span_of(p, b, a);
             const int64_t end = min(t1, s.hi);
             if (s.s < 0) {
                 Pack<T, V> none;
                 none.zero();
-                for (; a < end; ++a) none.store(db_out + a * p.channels);
+                for (; a < end; ++a) none.store(ob + a * p.channels);
                 continue;
             }
             const int64_t from = a, reach = min(min(p.len, s.hi), end + (W - 1));    // tokens whose g is needed
             Pack<T, V> nx[U], ng[U];
             load_group<T, V>(xb, p.xs[1], a, reach, nx);
             load_group<T, V>(gb, p.gs[1], a, reach, ng);
-            float in[W - 1 + U][V], g[W - 1 + U][V];    // inputs and gradients of tokens a - (W-1) ..
+            Lanes<V> in[W - 1 + U], g[W - 1 + U];       // inputs and gradients of tokens a - (W-1) ..
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) {
-                input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c, in[j]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[j][i] = 0.f;
+                in[j] = input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c);
+                g[j].zero();
             }
-            for (; a < end + (W - 1); a += U) {
-                float d[U][V];
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        in[W - 1 + k][i] = nx[k].get(i);
-                        d[k][i] = ng[k].get(i);
-                    }
-                load_group<T, V>(xb, p.xs[1], a + U, reach, nx);
-                load_group<T, V>(gb, p.gs[1], a + U, reach, ng);
-                const bool inner = a + U <= end;        // all four tokens are the piece's own
+            // One group.  INNER: its tokens are all the piece's own, and so are the W-1 before them.
+            auto group = [&](auto inner) {
+                constexpr bool INNER = decltype(inner)::value;
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
-                    const bool own = inner || a + k < end, has = inner || a + k < reach;
+                    Lanes<V> d;
+                    in[W - 1 + k].from(nx[k]);
+                    d.from(ng[k]);
+                    if (a + U + k < reach) {
+                        nx[k].load(xb + (a + U + k) * p.xs[1]);
+                        ng[k].load(gb + (a + U + k) * p.gs[1]);
+                    }
+                    const bool own = INNER || a + k < end, has = INNER || a + k < reach;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float o = f.bias[i];
+                    for (int i = 0; i < P; ++i) {
+                        F2 o = f.bias.v[i];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) o = fmaf(f.w[j][i], in[k + j][i], o);
-                        const float v = has ? pre_grad<T>(d[k][i], o, p.silu) : 0.f;
-                        g[W - 1 + k][i] = v;
+                        for (int j = 0; j < W; ++j) o = fma2(f.w[j].v[i], in[k + j].v[i], o);
+                        const F2 v = has ? pre_grad<T, SILU>(d.v[i], o) : F2(0.f);
+                        g[W - 1 + k].v[i] = v;
                         if (own) {
-                            db[i] += v;
+                            db.v[i] = fma2(v, F2(1.f), db.v[i]);
 #pragma unroll
-                            for (int j = 0; j < W; ++j) dw[j][i] = fmaf(v, in[k + j][i], dw[j][i]);
+                            for (int j = 0; j < W; ++j) dw[j].v[i] = fma2(v, in[k + j].v[i], dw[j].v[i]);
                         }
                     }
                     const int64_t u = a + k - (W - 1);  // all that u reaches is there: token u + m saw it through tap W-1-m
-                    if (u >= from && u < end) {
-                        float o[V];
+                    if (INNER || (u >= from && u < end)) {
+                        Lanes<V> o;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            o[i] = 0.f;
+                        for (int i = 0; i < P; ++i) {
+                            o.v[i] = mul2(f.w[W - 1].v[i], g[k].v[i]);
 #pragma unroll
-                            for (int m = 0; m < W; ++m) o[i] = fmaf(f.w[W - 1 - m][i], g[k + m][i], o[i]);
+                            for (int m = 1; m < W; ++m) o.v[i] = fma2(f.w[W - 1 - m].v[i], g[k + m].v[i], o.v[i]);
                         }
-                        if (dfin != nullptr && u >= s.hi - (W - 1)) {
-                            const T* q = dfin + ((int64_t)s.s * (W - 1) + (u - (s.hi - (W - 1)))) * p.channels + c;
+                        if (!INNER && dfin != nullptr && u >= s.hi - (W - 1)) {
+                            Pack<T, V> q;
+                            q.load(dfin + ((int64_t)s.s * (W - 1) + (u - (s.hi - (W - 1)))) * p.channels + c);
+                            Lanes<V> r;
+                            r.from(q);
 #pragma unroll
-                            for (int i = 0; i < V; ++i) o[i] += to_f<T>(q[i]);
+                            for (int i = 0; i < P; ++i) o.v[i] = fma2(r.v[i], F2(1.f), o.v[i]);
                         }
                         Pack<T, V> out;
-#pragma unroll
-                        for (int i = 0; i < V; ++i) out.set(i, o[i]);
-                        out.store(db_out + u * p.channels);
+                        o.to(out);
+                        out.store(ob + u * p.channels);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        in[j][i] = in[j + U][i];
-                        g[j][i] = g[j + U][i];
-                    }
+                for (int j = 0; j < W - 1; ++j) {
+                    in[j] = in[j + U];
+                    g[j] = g[j + U];
+                }
+            };
+            for (; a < end + (W - 1); a += U) {
+                if (a + U <= end && a >= from + (W - 1)) group(std::true_type());
+                else group(std::false_type());
             }
             a = end;
         }
@@ -303,8 +332,8 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, co
     for (int i = 0; i < V; ++i) {
         float* r = red + (int64_t)threadIdx.y * (W + 1) * width + threadIdx.x * V + i;
 #pragma unroll
-        for (int j = 0; j < W; ++j) r[j * width] = dw[j][i];
-        r[W * width] = db[i];
+        for (int j = 0; j < W; ++j) r[j * width] = i & 1 ? dw[j].v[i / 2].y() : dw[j].v[i / 2].x();
+        r[W * width] = i & 1 ? db.v[i / 2].y() : db.v[i / 2].x();
     }
     __syncthreads();
     const int64_t row = ((int64_t)b * gridDim.y + blockIdx.y) * (W + 1);
@@ -333,10 +362,9 @@ __global__ void __launch_bounds__(256) conv_init_grad_kernel(const ConvParams p,
     if (s.hi > p.len) s.hi = p.len;
     if (s.hi < s.lo) s.hi = s.lo;
     const int64_t b = p.cu != nullptr ? 0 : q;
-    float w[W], acc[W - 1], win[W][1];
-    const float bias = p.bias != nullptr ? param<T>(p, p.bias, c) : 0.f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j] = param<T>(p, p.w, (int64_t)c * W + j);
+    Filter<W, 1> f;
+    f.template load<T>(p, c);
+    float acc[W - 1];
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) {
         acc[r] = 0.f;
@@ -346,16 +374,16 @@ __global__ void __launch_bounds__(256) conv_init_grad_kernel(const ConvParams p,
     for (int n = 0; n < W - 1; ++n) {
         const int64_t t = s.lo + n;
         if (t >= s.hi) break;
-        float a = bias;
+        F2 o = f.bias.v[0];
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            input_of<T, W, 1>(p, x, init, s, b, t - (W - 1) + j, c, win[j]);
-            a = fmaf(w[j], win[j][0], a);
-        }
-        const float g = pre_grad<T>(to_f<T>(dy[b * p.gs[0] + t * p.gs[1] + c]), a, p.silu);
+        for (int j = 0; j < W; ++j) o = fma2(f.w[j].v[0], input_of<T, W, 1>(p, x, init, s, b, t - (W - 1) + j, c).v[0], o);
+        const F2 dv(to_f<T>(dy[b * p.gs[0] + t * p.gs[1] + c]), 0.f);
+        const float g = (p.silu ? pre_grad<T, true>(dv, o) : dv).x();
 #pragma unroll
         for (int r = 0; r < W - 1; ++r)             // tap j of token lo + n is row j + n
-            if (r - n >= 0) acc[r] = fmaf(w[r - n], g, acc[r]);
+#pragma unroll
+            for (int m = 0; m <= r; ++m)
+                if (m == n) acc[r] = fmaf(f.w[r - m].v[0].x(), g, acc[r]);
     }
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) dinit[(q * (W - 1) + r) * p.channels + c] = from_f<T>(acc[r]);
@@ -396,13 +424,20 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const ConvParams p, cons
     in.load(x + b * p.xs[0] + c);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) old[j].load(h + (int64_t)j * p.channels);
+    Filter<W, V> f;
+    f.template load<T>(p, c);
+    Lanes<V> o = f.bias, v;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float a = p.bias != nullptr ? param<T>(p, p.bias, c + i) : 0.f;
+    for (int j = 0; j < W; ++j) {
+        v.from(j < W - 1 ? old[j < W - 1 ? j : 0] : in);
 #pragma unroll
-        for (int j = 0; j < W; ++j) a = fmaf(param<T>(p, p.w, (int64_t)(c + i) * W + j), (j < W - 1 ? old[j].get(i) : in.get(i)), a);
-        out.set(i, activate<T>(a, p.silu));
+        for (int i = 0; i < Lanes<V>::P; ++i) o.v[i] = fma2(f.w[j].v[i], v.v[i], o.v[i]);
     }
+    if (p.silu) {
+#pragma unroll
+        for (int i = 0; i < Lanes<V>::P; ++i) o.v[i] = activate<T, true>(o.v[i]);
+    }
+    o.to(out);
 #pragma unroll
     for (int j = 0; j + 1 < W - 1; ++j) old[j + 1].store(h + (int64_t)j * p.channels);
     in.store(h + (int64_t)(W - 2) * p.channels);
@@ -432,8 +467,11 @@ Shape shape_of(const ConvParams& p, int v) {
     return s;
 }
 
+// Packs of v elements: every row on a boundary, the parameters too.
 bool vec_ok(const ConvParams& p, int v, int elem, const void* const* ptrs, int n) {
-    bool ok = p.channels % v == 0 && p.xs[0] % v == 0 && p.xs[1] % v == 0 && p.gs[0] % v == 0 && p.gs[1] % v == 0;
+    const int wide = p.w32 ? 4 * v : elem * v;
+    bool ok = fbla::seq::aligned_to(p.w, wide > 16 ? 16 : wide) && fbla::seq::aligned_to(p.bias, wide > 16 ? 16 : wide);
+    ok = ok && p.channels % v == 0 && p.xs[0] % v == 0 && p.xs[1] % v == 0 && p.gs[0] % v == 0 && p.gs[1] % v == 0;
     for (int i = 0; i < n; ++i) ok = ok && fbla::seq::aligned_to(ptrs[i], (int64_t)v * elem);
     return ok;
 }
@@ -474,14 +512,15 @@ template <typename T, int W, int V>
 cudaError_t launch_fwd(ConvParams p, const T* x, const T* init, T* y, cudaStream_t st) {
     const Shape s = shape_of(p, V);
     p.run = s.run;
-    conv_fwd_kernel<T, W, V><<<token_grid(p, s, V), dim3(s.vx, s.ty), 0, st>>>(p, x, init, y);
+    if (p.silu) conv_fwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), 0, st>>>(p, x, init, y);
+    else conv_fwd_kernel<T, W, V, false><<<token_grid(p, s, V), dim3(s.vx, s.ty), 0, st>>>(p, x, init, y);
     fbla::note_launches(1);
     return cudaGetLastError();
 }
 
 template <typename T, int W>
 cudaError_t run_fwd(const ConvParams& p, const T* x, const T* init, T* y, T* fin, cudaStream_t st) {
-    constexpr int V = 16 / (int)sizeof(T);
+    constexpr int V = 4;
     const void* ptrs[3] = {x, init, y};
     if (p.len > 0 && p.batch > 0) {
         const cudaError_t e = vec_ok(p, V, sizeof(T), ptrs, 3) ? launch_fwd<T, W, V>(p, x, init, y, st) : launch_fwd<T, W, 1>(p, x, init, y, st);
@@ -499,7 +538,8 @@ cudaError_t launch_bwd(ConvParams p, const T* x, const T* init, const T* dy, con
     const Shape s = shape_of(p, V);
     p.run = s.run;
     const size_t smem = (size_t)s.ty * (W + 1) * s.vx * V * sizeof(float);
-    conv_bwd_kernel<T, W, V><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
+    if (p.silu) conv_bwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
+    else conv_bwd_kernel<T, W, V, false><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
     fbla::note_launches(1);
     return cudaGetLastError();
 }
