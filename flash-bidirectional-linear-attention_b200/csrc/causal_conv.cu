@@ -9,8 +9,9 @@
 // What bounds it: HBM (forward one read and one write, backward two reads and one write).  Channels are
 // the contiguous dimension, so a thread owns V channels and walks along the tokens with the last W-1
 // inputs (and, backward, the last W-1 gradients) in registers: x is read once, plus W-1 tokens per run.
-// Tokens go by in groups of four, and the next group's loads are on their way while one is worked on: with
-// one load in flight per thread a B8-T4096-C2048 forward took 124 us and the backward 298.
+// Tokens go by in groups of four, and the groups to come are on their way (Ring below): with one load in flight
+// per thread a B8-T4096-C2048 forward took 124 us and the backward 298; with a group's loads in registers, where
+// the compiler decides what is waited for together, 66 and 214.
 // Two channels share the packed fp32 instructions: in plain ones the arithmetic (W products per element forward,
 // 3 W + 1 backward, a sigmoid) takes as long as the memory.  The weight gradient is summed in registers over a thread's run, in shared memory over the runs of a
 // block, and then over the blocks by a kernel of its own: no atomics, the same bits on every run.
@@ -125,12 +126,61 @@ template <typename T, bool SILU> __device__ __forceinline__ F2 pre_grad(F2 dy, F
 }
 
 constexpr int U = 4;            // tokens of a group
+constexpr int kStages = 3;      // groups in the ring
 
-template <typename T, int V> __device__ __forceinline__ void load_group(const T* base, int64_t stride, int64_t t, int64_t end, Pack<T, V> (&v)[U]) {
+// A thread's own tokens on their way from global memory: asynchronous copies into a ring of groups in shared
+// memory, two groups ahead.  A slot is written and read by one thread only, so nothing but that thread's own wait
+// orders it.  Copies are of 4 bytes or more; the one 2-byte case (odd channel counts of the 16-bit types) keeps
+// the next group in registers.
+template <typename T, int V> struct Ring {
+    static constexpr int kBytes = (int)sizeof(T) * V;
+    static constexpr bool kAsync = kBytes >= 4;
+    static constexpr int kAhead = kAsync ? kStages - 1 : 1;
+    static constexpr int kThreadBytes = kAsync ? kStages * U * kBytes : 0;
+    const T* base;
+    int64_t stride;
+    uint32_t at;                // shared address of this thread's first slot
+    Pack<T, V> regs[kAsync ? 1 : U];
+    __device__ __forceinline__ Ring(const T* b, int64_t s, unsigned char* smem) : base(b), stride(s) {
+        at = (uint32_t)__cvta_generic_to_shared(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * kBytes;
+    }
+    __device__ __forceinline__ uint32_t slot(int stage, int k) const { return at + (stage * U + k) * 256 * kBytes; }
+    // Tokens t .. t + U - 1 into `stage`, zeros from `end` on.
+    __device__ __forceinline__ void fetch(int stage, int64_t t, int64_t end) {
+        if constexpr (kAsync) {
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-        if (t + k < end) v[k].load(base + (t + k) * stride);
-}
+            for (int k = 0; k < U; ++k) {
+                const bool in = t + k < end;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(slot(stage, k)),
+                             "l"(base + (in ? t + k : 0) * stride), "n"(kBytes), "r"(in ? kBytes : 0) : "memory");
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                regs[k].zero();
+                if (t + k < end) regs[k].load(base + (t + k) * stride);
+            }
+        }
+    }
+    __device__ __forceinline__ Pack<T, V> get(int stage, int k) const {
+        Pack<T, V> r;
+        if constexpr (!kAsync) {
+            r = regs[k];
+        } else if constexpr (kBytes == 4) {
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&r)) : "r"(slot(stage, k)) : "memory");
+        } else if constexpr (kBytes == 8) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(slot(stage, k)) : "memory");
+        } else {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(slot(stage, k)) : "memory");
+        }
+        return r;
+    }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void ring_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Parameters of V channels
 template <int W, int V> struct Filter {
@@ -170,6 +220,8 @@ __global__ void __launch_bounds__(256, 2) conv_fwd_kernel(const ConvParams p, co
     T* yb = y + b * p.len * p.channels + c;
     Filter<W, V> f;
     f.template load<T>(p, c);
+    extern __shared__ __align__(16) unsigned char smem[];
+    Ring<T, V> rx(xb, p.xs[1], smem);
     for (int64_t a = t0; a < t1;) {
         const SeqSpan s = span_of(p, b, a);
         const int64_t end = min(t1, s.hi);
@@ -179,16 +231,24 @@ __global__ void __launch_bounds__(256, 2) conv_fwd_kernel(const ConvParams p, co
             for (; a < end; ++a) none.store(yb + a * p.channels);
             continue;
         }
-        Pack<T, V> next[U];
-        load_group<T, V>(xb, p.xs[1], a, end, next);
+#pragma unroll
+        for (int i = 0; i < Ring<T, V>::kAhead; ++i) {
+            rx.fetch(i, a + i * U, end);
+            ring_commit();
+        }
         Lanes<V> in[W - 1 + U];         // the last W-1 inputs, then the group's
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) in[j] = input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c);
-        for (; a < end; a += U) {
+        for (int stage = 0; a < end; a += U) {
+            ring_wait<Ring<T, V>::kAhead - 1>();
+#pragma unroll
+            for (int k = 0; k < U; ++k) in[W - 1 + k].from(rx.get(stage, k));
+            const int into = stage == 0 ? kStages - 1 : stage - 1;      // the slot read before this one
+            rx.fetch(into, a + Ring<T, V>::kAhead * U, end);
+            ring_commit();
+            stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                in[W - 1 + k].from(next[k]);
-                if (a + U + k < end) next[k].load(xb + (a + U + k) * p.xs[1]);
                 Lanes<V> o = f.bias;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
@@ -203,6 +263,7 @@ __global__ void __launch_bounds__(256, 2) conv_fwd_kernel(const ConvParams p, co
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) in[j] = in[j + U];
         }
+        ring_wait<0>();                 // the zeros behind the piece's end: the next piece starts the ring anew
         a = end;
     }
 }
@@ -232,7 +293,7 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, co
                                                           const T* __restrict__ dy, const T* __restrict__ dfin, T* __restrict__ dx,
                                                           float* __restrict__ part) {
     constexpr int P = Lanes<V>::P;
-    extern __shared__ float red[];              // [blockDim.y][W + 1][blockDim.x * V]
+    extern __shared__ __align__(16) unsigned char smem[];       // the rings of x and dy; then the block's sums
     const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
     const int64_t b = blockIdx.z;
     const int64_t t0 = ((int64_t)blockIdx.y * blockDim.y + threadIdx.y) * p.run;
@@ -247,6 +308,7 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, co
         T* ob = dx + b * p.len * p.channels + c;
         Filter<W, V> f;
         f.template load<T>(p, c);
+        Ring<T, V> rx(xb, p.xs[1], smem), rg(gb, p.gs[1], smem + 256 * Ring<T, V>::kThreadBytes);
         for (int64_t a = t0; a < t1;) {
             const SeqSpan s = span_of(p, b, a);
             const int64_t end = min(t1, s.hi);
@@ -257,27 +319,38 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, co
                 continue;
             }
             const int64_t from = a, reach = min(min(p.len, s.hi), end + (W - 1));    // tokens whose g is needed
-            Pack<T, V> nx[U], ng[U];
-            load_group<T, V>(xb, p.xs[1], a, reach, nx);
-            load_group<T, V>(gb, p.gs[1], a, reach, ng);
+#pragma unroll
+            for (int i = 0; i < Ring<T, V>::kAhead; ++i) {
+                rx.fetch(i, a + i * U, reach);
+                rg.fetch(i, a + i * U, reach);
+                ring_commit();
+            }
             Lanes<V> in[W - 1 + U], g[W - 1 + U];       // inputs and gradients of tokens a - (W-1) ..
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) {
                 in[j] = input_of<T, W, V>(p, x, init, s, b, a - (W - 1) + j, c);
                 g[j].zero();
             }
+            int stage = 0;
             // One group.  INNER: its tokens are all the piece's own, and so are the W-1 before them.
             auto group = [&](auto inner) {
                 constexpr bool INNER = decltype(inner)::value;
+                ring_wait<Ring<T, V>::kAhead - 1>();
+                Pack<T, V> pg[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    in[W - 1 + k].from(rx.get(stage, k));
+                    pg[k] = rg.get(stage, k);
+                }
+                const int into = stage == 0 ? kStages - 1 : stage - 1;      // the slot read before this one
+                rx.fetch(into, a + Ring<T, V>::kAhead * U, reach);
+                rg.fetch(into, a + Ring<T, V>::kAhead * U, reach);
+                ring_commit();
+                stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
                 for (int k = 0; k < U; ++k) {
                     Lanes<V> d;
-                    in[W - 1 + k].from(nx[k]);
-                    d.from(ng[k]);
-                    if (a + U + k < reach) {
-                        nx[k].load(xb + (a + U + k) * p.xs[1]);
-                        ng[k].load(gb + (a + U + k) * p.gs[1]);
-                    }
+                    d.from(pg[k]);
                     const bool own = INNER || a + k < end, has = INNER || a + k < reach;
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
@@ -324,9 +397,12 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const ConvParams p, co
                 if (a + U <= end && a >= from + (W - 1)) group(std::true_type());
                 else group(std::false_type());
             }
+            ring_wait<0>();             // the zeros behind the piece's reach: the next piece starts the rings anew
             a = end;
         }
     }
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(smem);        // [blockDim.y][W + 1][blockDim.x * V]
     const int width = blockDim.x * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -512,8 +588,10 @@ template <typename T, int W, int V>
 cudaError_t launch_fwd(ConvParams p, const T* x, const T* init, T* y, cudaStream_t st) {
     const Shape s = shape_of(p, V);
     p.run = s.run;
-    if (p.silu) conv_fwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), 0, st>>>(p, x, init, y);
-    else conv_fwd_kernel<T, W, V, false><<<token_grid(p, s, V), dim3(s.vx, s.ty), 0, st>>>(p, x, init, y);
+    const size_t smem = 256 * Ring<T, V>::kThreadBytes;
+    static_assert(256 * Ring<T, V>::kThreadBytes <= 48 * 1024, "the ring fits without asking for more");
+    if (p.silu) conv_fwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, y);
+    else conv_fwd_kernel<T, W, V, false><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, y);
     fbla::note_launches(1);
     return cudaGetLastError();
 }
@@ -537,7 +615,10 @@ template <typename T, int W, int V>
 cudaError_t launch_bwd(ConvParams p, const T* x, const T* init, const T* dy, const T* dfin, T* dx, float* part, cudaStream_t st) {
     const Shape s = shape_of(p, V);
     p.run = s.run;
-    const size_t smem = (size_t)s.ty * (W + 1) * s.vx * V * sizeof(float);
+    const size_t rings = 2 * 256 * Ring<T, V>::kThreadBytes, sums = (size_t)s.ty * (W + 1) * s.vx * V * sizeof(float);
+    const size_t smem = rings > sums ? rings : sums;
+    static_assert(2 * 256 * Ring<T, V>::kThreadBytes <= 48 * 1024 && 256 * (W + 1) * V * sizeof(float) <= 48 * 1024,
+                  "rings and sums fit without asking for more");
     if (p.silu) conv_bwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
     else conv_bwd_kernel<T, W, V, false><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
     fbla::note_launches(1);
