@@ -208,7 +208,7 @@ template <int W, int V> struct Filter {
 
 // A thread walks over its run piece by piece, a piece being the run's tokens of one sequence.
 template <typename T, int W, int V, bool SILU>
-__global__ void __launch_bounds__(256, 2) conv_fwd_kernel(const ConvParams p, const T* __restrict__ x, const T* __restrict__ init,
+__global__ void __launch_bounds__(256, 3) conv_fwd_kernel(const ConvParams p, const T* __restrict__ x, const T* __restrict__ init,
                                                           T* __restrict__ y) {
     constexpr int P = Lanes<V>::P;
     const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
@@ -527,15 +527,16 @@ struct Shape {
     int64_t blocks_t;       // blocks along the tokens
 };
 
-// Longer runs read fewer halo tokens, shorter ones give more threads.  A run of 32 costs (W-1)/32 = 9 %
-// more reads (mostly from L2); with fewer than about four warps per scheduler the latency of a run's
-// loads shows instead, so runs shrink until there are 148 * 1024 threads or four tokens are left.
+// Longer runs read fewer halo tokens and have fewer groups at their edges, shorter ones give more threads.  At
+// B8-T4096-C2048 runs of 64 tokens against 32: forward 55 us against 60, backward 108 against 125.  With fewer than
+// about four warps per scheduler the latency of a run's loads shows instead, so runs shrink until there are 148 * 1024
+// threads or four tokens are left.
 Shape shape_of(const ConvParams& p, int v) {
     Shape s;
     const int nv = (p.channels + v - 1) / v;
     s.vx = nv >= 64 ? 64 : (nv >= 32 ? 32 : 16);
     s.ty = 256 / s.vx;
-    s.run = 32;
+    s.run = 64;
     const int64_t per_token = (int64_t)p.batch * nv;
     while (s.run > 4 && per_token * ((p.len + s.run - 1) / s.run) < 148LL * 1024) s.run /= 2;
     while (p.len > 65535LL * s.run * s.ty) s.run *= 2;      // blocks along one grid dimension
@@ -615,8 +616,8 @@ template <typename T, int W, int V>
 cudaError_t launch_bwd(ConvParams p, const T* x, const T* init, const T* dy, const T* dfin, T* dx, float* part, cudaStream_t st) {
     const Shape s = shape_of(p, V);
     p.run = s.run;
-    const size_t rings = 2 * 256 * Ring<T, V>::kThreadBytes, sums = (size_t)s.ty * (W + 1) * s.vx * V * sizeof(float);
-    const size_t smem = rings > sums ? rings : sums;
+    const int rings = 2 * 256 * Ring<T, V>::kThreadBytes, sums = s.ty * (W + 1) * s.vx * V * (int)sizeof(float);
+    const int smem = rings > sums ? rings : sums;
     static_assert(2 * 256 * Ring<T, V>::kThreadBytes <= 48 * 1024 && 256 * (W + 1) * V * sizeof(float) <= 48 * 1024,
                   "rings and sums fit without asking for more");
     if (p.silu) conv_bwd_kernel<T, W, V, true><<<token_grid(p, s, V), dim3(s.vx, s.ty), smem, st>>>(p, x, init, dy, dfin, dx, part);
