@@ -572,9 +572,10 @@ int resolve(const fbla_conv_problem* p, ConvParams* r) {
     r->w32 = p->weight_dtype == FBLA_F32;
     r->num_seqs = p->cu_seqlens != nullptr ? p->num_seqs : p->batch;
     r->len = p->seq_len;
-    for (int i = 0; i < 2; ++i) {
-        r->xs[i] = p->x_stride[i];
-        r->gs[i] = p->dy_stride[i];
+    const int64_t size[2] = {p->batch, p->seq_len};
+    for (int i = 0; i < 2; ++i) {       // the stride of a dimension of one element is not used, whatever it is
+        r->xs[i] = size[i] > 1 ? p->x_stride[i] : 0;
+        r->gs[i] = size[i] > 1 ? p->dy_stride[i] : 0;
     }
     r->cu = p->cu_seqlens;
     r->run = 1;

@@ -171,7 +171,11 @@ cudaError_t dispatch(const RotaryParams& p, const void* q, const void* k, void* 
     auto fits = [&](int v) {
         const int64_t bytes = (int64_t)v * sizeof(T) > 16 ? 16 : (int64_t)v * sizeof(T);
         bool ok = p.dim % v == 0 && (p.interleaved || (p.pairs % v == 0));
-        for (int i = 0; i < 3; ++i) ok = ok && p.qs[i] % v == 0 && p.qos[i] % v == 0 && (p.hk == 0 || (p.ks[i] % v == 0 && p.kos[i] % v == 0));
+        const int64_t size[3] = {p.batch, p.hq, p.len}, size_k[3] = {p.batch, p.hk, p.len};     // a stride of one element is not used
+        for (int i = 0; i < 3; ++i) {
+            ok = ok && (size[i] == 1 || (p.qs[i] % v == 0 && p.qos[i] % v == 0));
+            ok = ok && (p.hk == 0 || size_k[i] == 1 || (p.ks[i] % v == 0 && p.kos[i] % v == 0));
+        }
         ok = ok && fbla::seq::aligned_to(q, bytes) && fbla::seq::aligned_to(qo, bytes);
         return ok && (p.hk == 0 || (fbla::seq::aligned_to(k, bytes) && fbla::seq::aligned_to(ko, bytes)));
     };

@@ -1004,11 +1004,12 @@ int resolve(const fbla_scan_problem* p, ScanParams* r) {
     r->softplus = p->softplus != 0;
     r->num_seqs = p->cu_seqlens != nullptr ? p->num_seqs : p->batch;
     r->len = p->seq_len;
-    for (int i = 0; i < 2; ++i) {
-        r->xs[i] = p->x_stride[i];
-        r->ds[i] = p->dt_stride[i];
-        r->zs[i] = p->z_stride[i];
-        r->gs[i] = p->dy_stride[i];
+    const int64_t size[2] = {p->batch, p->seq_len};
+    for (int i = 0; i < 2; ++i) {       // the stride of a dimension of one element is not used, whatever it is
+        r->xs[i] = size[i] > 1 ? p->x_stride[i] : 0;
+        r->ds[i] = size[i] > 1 ? p->dt_stride[i] : 0;
+        r->zs[i] = size[i] > 1 ? p->z_stride[i] : 0;
+        r->gs[i] = size[i] > 1 ? p->dy_stride[i] : 0;
     }
     for (int i = 0; i < 3; ++i) {
         r->bs[i] = p->b_stride[i];

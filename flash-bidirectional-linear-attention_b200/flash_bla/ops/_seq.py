@@ -14,10 +14,11 @@ def require_cuda(x):
         raise RuntimeError("flash_bla operators run on CUDA tensors only (there is no CPU path)")
 
 
-def same_device(x, **others):
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the first tensor on {x.device}")
+def same_device(x, *others):
+    d = x.device
+    for t in others:
+        if t is not None and t.device != d:
+            raise ValueError(f"all tensors must be on one device, got {d} and {t.device}")
 
 
 def check_cu_seqlens(cu):
@@ -28,12 +29,11 @@ def check_cu_seqlens(cu):
 
 def rows(t):
     """The tensor with its last dimension contiguous; the others may have any stride."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def stride(t, dim):
-    """Stride that the kernels see: a dimension of one element is never stepped over."""
-    return t.stride(dim) if t.shape[dim] > 1 else 0
+def dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def aligned(t):
@@ -42,7 +42,10 @@ def aligned(t):
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 def refuse_grad(what, *tensors):

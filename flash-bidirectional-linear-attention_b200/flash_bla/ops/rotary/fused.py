@@ -67,23 +67,23 @@ def rotary_frequencies(
     return freqs.repeat(axes).to(device), factor
 
 
-# order of (batch, head, token) in the tensor's dimensions
+# positions of (batch, head, token) among the tensor's dimensions; None: packed (total, heads, features)
 _DIMS = {"bhld": (0, 1, 2), "blhd": (0, 2, 1)}
 
 
-def _sizes(t, dims):
-    if dims is None:                        # packed (total, heads, features)
-        return 1, t.shape[1], t.shape[0]
-    return t.shape[dims[0]], t.shape[dims[1]], t.shape[dims[2]]
-
-
-def _strides(t, dims):
+def _order(v, dims):
+    """(batch, head, token) entries of a shape or of strides; a packed tensor has no batch."""
     if dims is None:
-        return 0, S.stride(t, 1), S.stride(t, 0)
-    return tuple(S.stride(t, d) for d in dims)
+        return None, v[1], v[0]
+    return v[dims[0]], v[dims[1]], v[dims[2]]
 
 
 _ZERO3 = (0, 0, 0)
+
+
+def _strides(v, dims):
+    b, h, t = _order(v, dims)
+    return b or 0, h, t
 
 
 def _rotate(q, k, freqs, positions, offset, factor, interleaved, axes, dims, cu, inverse):
@@ -91,20 +91,23 @@ def _rotate(q, k, freqs, positions, offset, factor, interleaved, axes, dims, cu,
     if q is None:
         return None, _rotate(k, None, freqs, positions, offset, factor, interleaved, axes, dims, cu, inverse)[0]
     q = S.rows(q)
-    k = None if k is None else S.rows(k)
     qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    B, H, L = _sizes(q, dims)
-    if positions is None:
-        pos32, pstride, pptr = 0, (0, 0), None
-    else:
-        pos32, pptr = int(positions.dtype == torch.int32), positions.data_ptr()
-        batched = positions.dim() - (axes > 1) == 2
-        pstride = (S.stride(positions, 0) if batched else 0, S.stride(positions, 1 if batched else 0))
-    prob = _C.RotaryProblem(_C.dtype_code(q.dtype), B, H, 0 if k is None else _sizes(k, dims)[1], q.shape[-1], freqs.numel(),
-                            axes, interleaved, inverse, pos32, 0 if cu is None else cu.numel() - 1, factor, L, offset,
-                            _strides(q, dims), _ZERO3 if k is None else _strides(k, dims), _strides(qo, dims),
-                            _ZERO3 if k is None else _strides(ko, dims), pstride, pptr, _C.ptr(cu), freqs.data_ptr())
+    B, H, L = _order(q.shape, dims)
+    Hk, ko, ks, kos = 0, None, _ZERO3, _ZERO3
+    if k is not None:
+        k = S.rows(k)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        Hk, ks, kos = _order(k.shape, dims)[1], _strides(k.stride(), dims), _strides(ko.stride(), dims)
+    pos32, pstride, pptr = 0, (0, 0), None
+    if positions is not None:
+        pos32, pptr, ps = positions.dtype == torch.int32, positions.data_ptr(), positions.stride()
+        if positions.dim() - (axes > 1) == 2:
+            pstride = (ps[0] if positions.shape[0] > 1 else 0, ps[1])
+        else:
+            pstride = (0, ps[0])
+    prob = _C.RotaryProblem(_C.dtype_code(q.dtype), 1 if B is None else B, H, Hk, q.shape[-1], freqs.numel(), axes, interleaved,
+                            inverse, pos32, 0 if cu is None else cu.numel() - 1, factor, L, offset, _strides(q.stride(), dims), ks,
+                            _strides(qo.stride(), dims), kos, pstride, pptr, _C.ptr(cu), freqs.data_ptr())
     S.call(_C.lib().fbla_rotary, prob, q, q.data_ptr(), _C.ptr(k), qo.data_ptr(), _C.ptr(ko))
     return qo, ko
 
@@ -169,13 +172,13 @@ def rotary_embedding(
         raise ValueError(f"expected q with {rank} dimensions in this layout, got shape {tuple(q.shape)}")
     if q.dtype not in S.FLOATS:
         raise TypeError(f"dtype {q.dtype} is not supported (float16, bfloat16, float32)")
-    B, H, L = _sizes(q, dims)
+    B, H, L = _order(q.shape, dims)
     if k is not None:
-        if k.dim() != rank or k.shape[-1] != q.shape[-1] or (_sizes(k, dims)[0], _sizes(k, dims)[2]) != (B, L):
+        if k.dim() != rank or k.shape[-1] != q.shape[-1] or _order(k.shape, dims)[0::2] != (B, L):
             raise ValueError(f"q and k must agree in all but the heads, got {tuple(q.shape)} and {tuple(k.shape)}")
         if k.dtype != q.dtype:
             raise ValueError("q and k must have the same dtype")
-        if k.shape[0 if dims is None else dims[1]] == 0:
+        if _order(k.shape, dims)[1] == 0:
             raise ValueError("k has no heads: pass None")
     if H == 0:
         raise ValueError("q has no heads")
@@ -195,13 +198,13 @@ def rotary_embedding(
         if offset != 0:
             raise ValueError("offset goes with positions=None")
         tail = (axes,) if axes > 1 else ()
-        if tuple(positions.shape) not in ((L,) + tail, (B, L) + tail, (1, L) + tail):
-            raise ValueError(f"positions of shape {tuple(positions.shape)} do not fit {B} rows of {L} tokens on {axes} axes")
+        if positions.shape not in ((L,) + tail, (B, L) + tail, (1, L) + tail):
+            raise ValueError(f"positions of shape {tuple(positions.shape)} do not fit {B or 1} rows of {L} tokens on {axes} axes")
         if axes > 1:
             positions = S.rows(positions)
-    S.same_device(q, k=k, freqs=freqs, positions=positions, cu_seqlens=cu_seqlens)
+    S.same_device(q, k, freqs, positions, cu_seqlens)
     S.require_cuda(q)
-    args = (freqs.contiguous(), positions, int(offset), float(factor), bool(interleaved), int(axes), dims, cu_seqlens)
+    args = (S.dense(freqs), positions, int(offset), float(factor), bool(interleaved), int(axes), dims, cu_seqlens)
     if S.wants_grad(q, k):
         qo, ko = RotaryFunction.apply(q, k, *args)
     else:

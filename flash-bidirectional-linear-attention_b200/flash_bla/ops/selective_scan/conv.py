@@ -30,14 +30,18 @@ def _check_weight(x, weight, bias, activation):
         raise ValueError(f"activation must be None or 'silu', got {activation!r}")
 
 
+def _lead(t):
+    """(batch, token) strides; a packed tensor has no batch."""
+    if t is None:
+        return 0, 0
+    s = t.stride()
+    return (s[0], s[1]) if len(s) == 3 else (0, s[0])
+
+
 def _problem(x, weight, silu, cu, dy=None):
-    if x.dim() == 3:
-        batch, length, xs = x.shape[0], x.shape[1], (S.stride(x, 0), S.stride(x, 1))
-    else:
-        batch, length, xs = 1, x.shape[0], (0, S.stride(x, 0))
-    gs = (0, 0) if dy is None else (S.stride(dy, 0), S.stride(dy, 1)) if dy.dim() == 3 else (0, S.stride(dy, 0))
-    return _C.ConvProblem(_C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), batch, x.shape[-1], weight.shape[1], silu,
-                          0 if cu is None else cu.numel() - 1, 0, length, xs, gs, _C.ptr(cu))
+    shape = x.shape
+    return _C.ConvProblem(_C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), shape[0] if len(shape) == 3 else 1, shape[-1],
+                          weight.shape[1], silu, 0 if cu is None else cu.numel() - 1, 0, shape[-2], _lead(x), _lead(dy), _C.ptr(cu))
 
 
 def _forward(x, weight, bias, state, silu, want_final, cu):
@@ -65,7 +69,7 @@ class CausalConv1dFunction(torch.autograd.Function):
     def backward(ctx, dy, dfinal):
         x, weight, bias, state, cu = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
-        dfinal = None if dfinal is None else dfinal.contiguous()
+        dfinal = S.dense(dfinal)
         prob = _problem(x, weight, ctx.silu, cu, dy)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dw = torch.empty_like(weight)
@@ -117,11 +121,10 @@ def causal_conv1d(
     if initial_state is not None:
         if tuple(initial_state.shape) != (rows, weight.shape[1] - 1, x.shape[-1]) or initial_state.dtype != x.dtype:
             raise ValueError(f"initial_state must have shape {(rows, weight.shape[1] - 1, x.shape[-1])} and the dtype of x")
-        initial_state = initial_state.contiguous()
-    S.same_device(x, weight=weight, bias=bias, initial_state=initial_state, cu_seqlens=cu_seqlens)
+        initial_state = S.dense(initial_state)
+    S.same_device(x, weight, bias, initial_state, cu_seqlens)
     S.require_cuda(x)
-    args = (S.rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), initial_state, activation == "silu",
-            bool(return_final_state), cu_seqlens)
+    args = (S.rows(x), S.dense(weight), S.dense(bias), initial_state, activation == "silu", bool(return_final_state), cu_seqlens)
     y, final = CausalConv1dFunction.apply(*args) if S.wants_grad(x, weight, bias, initial_state) else _forward(*args)
     return (y, final) if return_final_state else y
 
@@ -140,21 +143,21 @@ def causal_conv1d_step(
     if x.dim() != 2:
         raise ValueError(f"x must have shape (B, C), got {tuple(x.shape)}")
     _check_weight(x, weight, bias, activation)
-    if tuple(state.shape) != (x.shape[0], weight.shape[1] - 1, x.shape[1]) or state.dtype != x.dtype:
+    if state.shape != (x.shape[0], weight.shape[1] - 1, x.shape[1]) or state.dtype != x.dtype:
         raise ValueError(f"state must have shape {(x.shape[0], weight.shape[1] - 1, x.shape[1])} and the dtype of x")
     if not state.is_contiguous():
         raise ValueError("state is updated in place and must be contiguous")
     if x.shape[0] > 65535:
         raise ValueError(f"at most 65535 rows, got {x.shape[0]}")
-    S.same_device(x, state=state, weight=weight, bias=bias)
+    S.same_device(x, state, weight, bias)
     S.refuse_grad("causal_conv1d_step", x, state, weight, bias)
     S.require_cuda(x)
-    x, weight, bias = S.rows(x), weight.contiguous(), None if bias is None else bias.contiguous()
+    x, weight, bias = S.rows(x), S.dense(weight), S.dense(bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel() == 0:
         return y
     prob = _C.ConvProblem(_C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), x.shape[0], x.shape[1], weight.shape[1],
-                          activation == "silu", 0, 0, 1, (S.stride(x, 0), 0))
+                          activation == "silu", 0, 0, 1, (x.stride(0), 0))
     S.call(_C.lib().fbla_causal_conv_step, prob, x, x.data_ptr(), weight.data_ptr(), _C.ptr(bias),
            state.data_ptr(), y.data_ptr())
     return y

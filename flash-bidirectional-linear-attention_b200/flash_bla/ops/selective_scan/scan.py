@@ -18,29 +18,33 @@ from flash_bla.ops import _seq as S
 
 
 def _check(x, dt, A, B, C, D, z, dt_bias, lead):
-    """``lead``: the leading dimensions of x without the channels."""
-    ch = x.shape[-1]
-    if x.dtype not in S.FLOATS:
-        raise TypeError(f"dtype {x.dtype} is not supported (float16, bfloat16, float32)")
+    """``lead``: the number of x's dimensions before the channels.  Returns the number of groups."""
+    shape, dtype = x.shape, x.dtype
+    ch = shape[-1]
+    if dtype not in S.FLOATS:
+        raise TypeError(f"dtype {dtype} is not supported (float16, bfloat16, float32)")
     if ch == 0:
         raise ValueError("x has no channels")
-    for name, t in (("dt", dt), ("z", z)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must have the shape and the dtype of x, got {tuple(t.shape)} {t.dtype}")
+    if dt.shape != shape or dt.dtype != dtype:
+        raise ValueError(f"dt must have the shape and the dtype of x, got {tuple(dt.shape)} {dt.dtype}")
+    if z is not None and (z.shape != shape or z.dtype != dtype):
+        raise ValueError(f"z must have the shape and the dtype of x, got {tuple(z.shape)} {z.dtype}")
     if A.dim() != 2 or A.shape[0] != ch or A.dtype != torch.float32:
         raise ValueError("A must be a float32 tensor of shape (channels, states)")
-    if not 1 <= A.shape[1] <= 32:
-        raise ValueError(f"the number of states must be between 1 and 32, got {A.shape[1]}")
-    for name, t in (("B", B), ("C", C)):
-        if t.dtype != x.dtype or t.shape[:lead] != x.shape[:lead] or t.dim() not in (lead + 1, lead + 2) or t.shape[-1] != A.shape[1]:
-            raise ValueError(f"{name} must have the dtype of x and shape (..., states) or (..., groups, states), got {tuple(t.shape)}")
-    if B.shape != C.shape:
+    N = A.shape[1]
+    if not 1 <= N <= 32:
+        raise ValueError(f"the number of states must be between 1 and 32, got {N}")
+    bc = B.shape
+    for name, t, s in (("B", B, bc), ("C", C, C.shape)):
+        if t.dtype != dtype or len(s) not in (lead + 1, lead + 2) or s[:lead] != shape[:lead] or s[-1] != N:
+            raise ValueError(f"{name} must have the dtype of x and shape (..., states) or (..., groups, states), got {tuple(s)}")
+    if C.shape != bc:
         raise ValueError("B and C must have the same shape")
-    groups = B.shape[lead] if B.dim() == lead + 2 else 1
+    groups = bc[lead] if len(bc) == lead + 2 else 1
     if groups < 1 or ch % groups:
         raise ValueError(f"{groups} groups do not divide {ch} channels")
     for name, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None and (t.shape != x.shape[-1:] or t.dtype != torch.float32):
+        if t is not None and (t.shape != (ch,) or t.dtype != torch.float32):
             raise ValueError(f"{name} must be a float32 tensor of shape (channels,)")
     return groups
 
@@ -49,20 +53,23 @@ def _s2(t):
     """(batch, token) strides of x and the like; a packed tensor has no batch."""
     if t is None:
         return 0, 0
-    return (S.stride(t, 0), S.stride(t, 1)) if t.dim() == 3 else (0, S.stride(t, 0))
+    s = t.stride()
+    return (s[0], s[1]) if len(s) == 3 else (0, s[0])
 
 
 def _s3(t, lead):
     """(batch, token, group) strides of B, C."""
-    group = S.stride(t, lead) if t.dim() == lead + 2 else 0
-    return (S.stride(t, 0), S.stride(t, 1), group) if lead == 2 else (0, S.stride(t, 0), group)
+    s = t.stride()
+    group = s[lead] if len(s) == lead + 2 else 0
+    return (s[0], s[1], group) if lead == 2 else (0, s[0], group)
 
 
 def _problem(x, dt, A, B, C, z, softplus, cu, dy=None):
-    lead = x.dim() - 1
+    shape = x.shape
+    lead = len(shape) - 1
     groups = B.shape[lead] if B.dim() == lead + 2 else 1
-    return _C.ScanProblem(_C.dtype_code(x.dtype), x.shape[0] if lead == 2 else 1, x.shape[-1], A.shape[1], groups, softplus,
-                          0 if cu is None else cu.numel() - 1, 0, x.shape[lead - 1], _s2(x), _s2(dt), _s2(z), _s2(dy),
+    return _C.ScanProblem(_C.dtype_code(x.dtype), shape[0] if lead == 2 else 1, shape[-1], A.shape[1], groups, softplus,
+                          0 if cu is None else cu.numel() - 1, 0, shape[lead - 1], _s2(x), _s2(dt), _s2(z), _s2(dy),
                           _s3(B, lead), _s3(C, lead), _C.ptr(cu))
 
 
@@ -96,7 +103,7 @@ class SelectiveScanFunction(torch.autograd.Function):
     def backward(ctx, dy, dfinal):
         x, dt, A, B, C, D, z, dt_bias, state, cu, ckpt = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
-        dfinal = None if dfinal is None else S.aligned(dfinal.contiguous())
+        dfinal = S.aligned(S.dense(dfinal))
         prob = _problem(x, dt, A, B, C, z, ctx.softplus, cu, dy)
         new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
         dx, ddt, dA, dB, dC, dD, dz, dbias = (new(t) for t in (x, dt, A, B, C, D, z, dt_bias))
@@ -156,12 +163,11 @@ def selective_scan(
     if initial_state is not None:
         if tuple(initial_state.shape) != (rows,) + tuple(A.shape) or initial_state.dtype != torch.float32:
             raise ValueError(f"initial_state must be a float32 tensor of shape {(rows,) + tuple(A.shape)}")
-        initial_state = S.aligned(initial_state.contiguous())
-    S.same_device(x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, initial_state=initial_state, cu_seqlens=cu_seqlens)
+        initial_state = S.aligned(S.dense(initial_state))
+    S.same_device(x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
     S.require_cuda(x)
-    one = lambda t: None if t is None else t.contiguous()  # noqa: E731
-    args = (S.rows(x), S.rows(dt), A.contiguous(), S.rows(B), S.rows(C), one(D), None if z is None else S.rows(z), one(dt_bias),
-            initial_state, bool(dt_softplus), bool(return_final_state), cu_seqlens)
+    args = (S.rows(x), S.rows(dt), S.dense(A), S.rows(B), S.rows(C), S.dense(D), S.rows(z), S.dense(dt_bias), initial_state,
+            bool(dt_softplus), bool(return_final_state), cu_seqlens)
     if S.wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
         y, final = SelectiveScanFunction.apply(*args)
     else:
@@ -188,26 +194,24 @@ def selective_scan_step(
     if x.dim() != 2:
         raise ValueError(f"x must have shape (B, C), got {tuple(x.shape)}")
     groups = _check(x, dt, A, B, C, D, z, dt_bias, 1)
-    if tuple(state.shape) != (x.shape[0],) + tuple(A.shape) or state.dtype != torch.float32:
+    if state.shape != (x.shape[0],) + A.shape or state.dtype != torch.float32:
         raise ValueError(f"state must be a float32 tensor of shape {(x.shape[0],) + tuple(A.shape)}")
     if not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state is updated in place and must be contiguous and 16-byte aligned")
     if x.shape[0] > 65535:
         raise ValueError(f"at most 65535 rows, got {x.shape[0]}")
-    S.same_device(x, dt=dt, A=A, B=B, C=C, state=state, D=D, z=z, dt_bias=dt_bias)
+    S.same_device(x, dt, A, B, C, state, D, z, dt_bias)
     S.refuse_grad("selective_scan_step", x, dt, A, B, C, state, D, z, dt_bias)
     S.require_cuda(x)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel() == 0:
         return y
-    x, dt, B, C, A = S.rows(x), S.rows(dt), S.rows(B), S.rows(C), A.contiguous()
-    z = None if z is None else S.rows(z)
-    one = lambda t: None if t is None else t.contiguous()  # noqa: E731
-    D, dt_bias = one(D), one(dt_bias)
-    row = lambda t: (0, 0) if t is None else (S.stride(t, 0), 0)  # noqa: E731
-    group = lambda t: (S.stride(t, 0), 0, S.stride(t, 1) if t.dim() == 3 else 0)  # noqa: E731
-    prob = _C.ScanProblem(_C.dtype_code(x.dtype), x.shape[0], x.shape[1], A.shape[1], groups, dt_softplus, 0, 0, 1, row(x), row(dt),
-                          row(z), (0, 0), group(B), group(C))
+    x, dt, B, C, z, A = S.rows(x), S.rows(dt), S.rows(B), S.rows(C), S.rows(z), S.dense(A)
+    D, dt_bias = S.dense(D), S.dense(dt_bias)
+    bs, cs = B.stride(), C.stride()
+    prob = _C.ScanProblem(_C.dtype_code(x.dtype), x.shape[0], x.shape[1], A.shape[1], groups, dt_softplus, 0, 0, 1,
+                          (x.stride(0), 0), (dt.stride(0), 0), (0 if z is None else z.stride(0), 0), (0, 0),
+                          (bs[0], 0, bs[1] if len(bs) == 3 else 0), (cs[0], 0, cs[1] if len(cs) == 3 else 0))
     S.call(_C.lib().fbla_selective_scan_step, prob, x, x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
            _C.ptr(D), _C.ptr(z), _C.ptr(dt_bias), state.data_ptr(), y.data_ptr())
     return y
