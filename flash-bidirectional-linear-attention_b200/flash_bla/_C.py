@@ -72,28 +72,32 @@ class PeerGroup(ctypes.Structure):
 _i32, _i64 = ctypes.c_int32, ctypes.c_int64
 
 
+def _strides(*names):
+    """The header's stride arrays as single fields (the same layout): a nested array costs a microsecond per call."""
+    return [(f"{n}_stride{i}", _i64) for n, k in names for i in range(k)]
+
+
 class RotaryProblem(ctypes.Structure):
     """Mirror of ``struct fbla_rotary_problem``."""
     _fields_ = [(n, _i32) for n in ("dtype", "batch", "heads_q", "heads_k", "dim", "pairs", "axes", "interleaved",
                                     "inverse", "positions32", "num_seqs")]
     _fields_ += [("factor", ctypes.c_float), ("seq_len", _i64), ("offset", _i64)]
-    _fields_ += [(n, _i64 * 3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")]
-    _fields_ += [("pos_stride", _i64 * 2), ("positions", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+    _fields_ += _strides(("q", 3), ("k", 3), ("q_out", 3), ("k_out", 3), ("pos", 2))
+    _fields_ += [("positions", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
                  ("freqs", ctypes.c_void_p)]
 
 
 class ConvProblem(ctypes.Structure):
     """Mirror of ``struct fbla_conv_problem``."""
     _fields_ = [(n, _i32) for n in ("dtype", "weight_dtype", "batch", "channels", "width", "silu", "num_seqs", "reserved")]
-    _fields_ += [("seq_len", _i64), ("x_stride", _i64 * 2), ("dy_stride", _i64 * 2), ("cu_seqlens", ctypes.c_void_p)]
+    _fields_ += [("seq_len", _i64)] + _strides(("x", 2), ("dy", 2)) + [("cu_seqlens", ctypes.c_void_p)]
 
 
 class ScanProblem(ctypes.Structure):
     """Mirror of ``struct fbla_scan_problem``."""
     _fields_ = [(n, _i32) for n in ("dtype", "batch", "channels", "states", "groups", "softplus", "num_seqs", "reserved")]
-    _fields_ += [("seq_len", _i64)]
-    _fields_ += [(n, _i64 * 2) for n in ("x_stride", "dt_stride", "z_stride", "dy_stride")]
-    _fields_ += [("b_stride", _i64 * 3), ("c_stride", _i64 * 3), ("cu_seqlens", ctypes.c_void_p)]
+    _fields_ += [("seq_len", _i64)] + _strides(("x", 2), ("dt", 2), ("z", 2), ("dy", 2), ("b", 3), ("c", 3))
+    _fields_ += [("cu_seqlens", ctypes.c_void_p)]
 
 
 _P = ctypes.POINTER(Problem)

@@ -36,6 +36,13 @@ def dense(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+def new(t):
+    """A contiguous tensor of the shape, dtype and device of ``t``."""
+    if t is None:
+        return None
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def aligned(t):
     """States are read 16 bytes at a time: a view at an odd offset is copied."""
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()

@@ -91,12 +91,12 @@ def _rotate(q, k, freqs, positions, offset, factor, interleaved, axes, dims, cu,
     if q is None:
         return None, _rotate(k, None, freqs, positions, offset, factor, interleaved, axes, dims, cu, inverse)[0]
     q = S.rows(q)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    qo = S.new(q)
     B, H, L = _order(q.shape, dims)
     Hk, ko, ks, kos = 0, None, _ZERO3, _ZERO3
     if k is not None:
         k = S.rows(k)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        ko = S.new(k)
         Hk, ks, kos = _order(k.shape, dims)[1], _strides(k.stride(), dims), _strides(ko.stride(), dims)
     pos32, pstride, pptr = 0, (0, 0), None
     if positions is not None:
@@ -106,8 +106,8 @@ def _rotate(q, k, freqs, positions, offset, factor, interleaved, axes, dims, cu,
         else:
             pstride = (0, ps[0])
     prob = _C.RotaryProblem(_C.dtype_code(q.dtype), 1 if B is None else B, H, Hk, q.shape[-1], freqs.numel(), axes, interleaved,
-                            inverse, pos32, 0 if cu is None else cu.numel() - 1, factor, L, offset, _strides(q.stride(), dims), ks,
-                            _strides(qo.stride(), dims), kos, pstride, pptr, _C.ptr(cu), freqs.data_ptr())
+                            inverse, pos32, 0 if cu is None else cu.numel() - 1, factor, L, offset, *_strides(q.stride(), dims), *ks,
+                            *_strides(qo.stride(), dims), *kos, *pstride, pptr, _C.ptr(cu), freqs.data_ptr())
     S.call(_C.lib().fbla_rotary, prob, q, q.data_ptr(), _C.ptr(k), qo.data_ptr(), _C.ptr(ko))
     return qo, ko
 

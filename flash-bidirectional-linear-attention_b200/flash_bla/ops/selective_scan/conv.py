@@ -41,11 +41,11 @@ def _lead(t):
 def _problem(x, weight, silu, cu, dy=None):
     shape = x.shape
     return _C.ConvProblem(_C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), shape[0] if len(shape) == 3 else 1, shape[-1],
-                          weight.shape[1], silu, 0 if cu is None else cu.numel() - 1, 0, shape[-2], _lead(x), _lead(dy), _C.ptr(cu))
+                          weight.shape[1], silu, 0 if cu is None else cu.numel() - 1, 0, shape[-2], *_lead(x), *_lead(dy), _C.ptr(cu))
 
 
 def _forward(x, weight, bias, state, silu, want_final, cu):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = S.new(x)
     prob = _problem(x, weight, silu, cu)
     rows = prob.batch if cu is None else prob.num_seqs
     final = torch.empty(rows, weight.shape[1] - 1, x.shape[-1], dtype=x.dtype, device=x.device) if want_final else None
@@ -71,7 +71,7 @@ class CausalConv1dFunction(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.dense(dfinal)
         prob = _problem(x, weight, ctx.silu, cu, dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = S.new(x)
         dw = torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
@@ -153,11 +153,11 @@ def causal_conv1d_step(
     S.refuse_grad("causal_conv1d_step", x, state, weight, bias)
     S.require_cuda(x)
     x, weight, bias = S.rows(x), S.dense(weight), S.dense(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = S.new(x)
     if y.numel() == 0:
         return y
     prob = _C.ConvProblem(_C.dtype_code(x.dtype), _C.dtype_code(weight.dtype), x.shape[0], x.shape[1], weight.shape[1],
-                          activation == "silu", 0, 0, 1, (x.stride(0), 0))
+                          activation == "silu", 0, 0, 1, x.stride(0))
     S.call(_C.lib().fbla_causal_conv_step, prob, x, x.data_ptr(), weight.data_ptr(), _C.ptr(bias),
            state.data_ptr(), y.data_ptr())
     return y

@@ -69,14 +69,14 @@ def _problem(x, dt, A, B, C, z, softplus, cu, dy=None):
     lead = len(shape) - 1
     groups = B.shape[lead] if B.dim() == lead + 2 else 1
     return _C.ScanProblem(_C.dtype_code(x.dtype), shape[0] if lead == 2 else 1, shape[-1], A.shape[1], groups, softplus,
-                          0 if cu is None else cu.numel() - 1, 0, shape[lead - 1], _s2(x), _s2(dt), _s2(z), _s2(dy),
-                          _s3(B, lead), _s3(C, lead), _C.ptr(cu))
+                          0 if cu is None else cu.numel() - 1, 0, shape[lead - 1], *_s2(x), *_s2(dt), *_s2(z),
+                          *_s2(dy), *_s3(B, lead), *_s3(C, lead), _C.ptr(cu))
 
 
 def _forward(x, dt, A, B, C, D, z, dt_bias, state, softplus, want_final, cu, checkpoints=False):
     L = _C.lib()
     prob = _problem(x, dt, A, B, C, z, softplus, cu)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = S.new(x)
     rows = prob.batch if cu is None else prob.num_seqs
     final = torch.empty(rows, *A.shape, dtype=torch.float32, device=x.device) if want_final else None
     ckpt = None
@@ -105,9 +105,8 @@ class SelectiveScanFunction(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.aligned(S.dense(dfinal))
         prob = _problem(x, dt, A, B, C, z, ctx.softplus, cu, dy)
-        new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        dx, ddt, dA, dB, dC, dD, dz, dbias = (new(t) for t in (x, dt, A, B, C, D, z, dt_bias))
-        dstate = new(state) if ctx.needs_input_grad[8] else None
+        dx, ddt, dA, dB, dC, dD, dz, dbias = (S.new(t) for t in (x, dt, A, B, C, D, z, dt_bias))
+        dstate = S.new(state) if ctx.needs_input_grad[8] else None
         L = _C.lib()
         ws, n = S.scratch(L.fbla_selective_scan_workspace_bytes(ctypes.byref(prob), 1), x)
         S.call(L.fbla_selective_scan_bwd, prob, x, x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _C.ptr(D),
@@ -203,15 +202,15 @@ def selective_scan_step(
     S.same_device(x, dt, A, B, C, state, D, z, dt_bias)
     S.refuse_grad("selective_scan_step", x, dt, A, B, C, state, D, z, dt_bias)
     S.require_cuda(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = S.new(x)
     if y.numel() == 0:
         return y
     x, dt, B, C, z, A = S.rows(x), S.rows(dt), S.rows(B), S.rows(C), S.rows(z), S.dense(A)
     D, dt_bias = S.dense(D), S.dense(dt_bias)
     bs, cs = B.stride(), C.stride()
     prob = _C.ScanProblem(_C.dtype_code(x.dtype), x.shape[0], x.shape[1], A.shape[1], groups, dt_softplus, 0, 0, 1,
-                          (x.stride(0), 0), (dt.stride(0), 0), (0 if z is None else z.stride(0), 0), (0, 0),
-                          (bs[0], 0, bs[1] if len(bs) == 3 else 0), (cs[0], 0, cs[1] if len(cs) == 3 else 0))
+                          x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, 0, 0,
+                          bs[0], 0, bs[1] if len(bs) == 3 else 0, cs[0], 0, cs[1] if len(cs) == 3 else 0)
     S.call(_C.lib().fbla_selective_scan_step, prob, x, x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
            _C.ptr(D), _C.ptr(z), _C.ptr(dt_bias), state.data_ptr(), y.data_ptr())
     return y

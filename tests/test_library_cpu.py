@@ -118,3 +118,11 @@ def test_naive_statements_match_the_oracle():
     cu = torch.tensor([0, 5, 20, 33], dtype=torch.int32)
     qq, kk, vv = q[0].transpose(0, 1).contiguous(), k[0].transpose(0, 1).contiguous(), v[0].transpose(0, 1).contiguous()
     assert torch.allclose(naive_varlen_linear_attn(qq, kk, vv, cu), O.varlen_linear_attn_fwd(qq, kk, vv, cu), atol=1e-12)
+
+
+def test_sequence_problem_structs_match_header_layout():
+    """Sizes and the offsets behind each run of 4-byte fields, as the C compiler lays the header's structs out."""
+    R, V, S = _C.RotaryProblem, _C.ConvProblem, _C.ScanProblem
+    assert ctypes.sizeof(R) == 200 and R.factor.offset == 44 and R.seq_len.offset == 48 and R.pos_stride0.offset == 160
+    assert ctypes.sizeof(V) == 80 and V.seq_len.offset == 32 and V.cu_seqlens.offset == 72
+    assert ctypes.sizeof(S) == 160 and S.seq_len.offset == 32 and S.b_stride0.offset == 104 and S.cu_seqlens.offset == 152
