@@ -8,8 +8,7 @@
 // What bounds it: HBM, one read and one write of q and k.  The angle of a (token, pair) is the same for
 // all heads, so a thread owns a few pairs of one token, forms their sines once and walks over the heads,
 // four at a time so that eight loads are in flight.  Angles are reduced in 64 bits (a position of 1e6
-// leaves only 2^-4 of a turn in fp32 products): turns = pos * freq / 2pi, minus the nearest integer, then
-// sincospi in fp32.
+// leaves only 2^-4 of a turn in fp32 products).
 #include <cmath>
 
 #include "seq_common.cuh"
@@ -32,6 +31,20 @@ struct RotaryParams {
     const double* freqs;
     float factor, sign;
 };
+
+// Sine and cosine of an angle in turns, reduced to half a turn in 64 bits: adding and taking away 1.5 * 2^52 rounds
+// to the nearest integer.  fp32 results: to two units in the last place; 16-bit ones: the special function unit's,
+// 2^-21 absolute, far below their rounding (forming them otherwise costs more than a dozen heads' products).
+template <typename T> __device__ __forceinline__ void sincos_turns(double turns, float& s, float& c) {
+    const double whole = __dadd_rn(__dadd_rn(turns, 6755399441055744.0), -6755399441055744.0);
+    const float f = (float)(turns - whole);
+    if (sizeof(T) == 4) {
+        sincospif(2.f * f, &s, &c);
+    } else {
+        s = __sinf(f * 6.28318531f);
+        c = __cosf(f * 6.28318531f);
+    }
+}
 
 // Slots of one token: PAIRED = two runs of V features whose elements pair up (half layout, and V = 1 for
 // interleaved pairs at odd alignments); otherwise one run of V features holding V/2 interleaved pairs.
@@ -59,24 +72,23 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const
     if (!copy) {
         const int pair0 = PAIRED ? slot * V : slot * NP;
         const int per_axis = p.pairs / p.axes;
+        auto position = [&](int axis) {
+            if (p.positions == nullptr) return (double)(t - start + p.offset);
+            const int64_t at = b * p.pos_b + t * p.pos_t + axis;
+            return p.positions32 ? (double)reinterpret_cast<const int32_t*>(p.positions)[at]
+                                 : (double)reinterpret_cast<const int64_t*>(p.positions)[at];
+        };
+        int axis = pair0 / per_axis;
+        double pos = pair0 < p.pairs ? position(axis) * 0.15915494309189533577 : 0.0;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int pr = pair0 + j;
             cs[j] = 1.f;
             sn[j] = 0.f;
             if (pr < p.pairs) {
-                int64_t pos;
-                if (p.positions == nullptr) {
-                    pos = t - start + p.offset;
-                } else {
-                    const int64_t at = b * p.pos_b + t * p.pos_t + (p.axes > 1 ? pr / per_axis : 0);
-                    pos = p.positions32 ? (int64_t) reinterpret_cast<const int32_t*>(p.positions)[at]
-                                        : reinterpret_cast<const int64_t*>(p.positions)[at];
-                }
-                double turns = (double)pos * (p.freqs[pr] * 0.15915494309189533577);
-                turns -= rint(turns);
+                if (p.axes > 1 && pr >= (axis + 1) * per_axis) pos = position(++axis) * 0.15915494309189533577;
                 float s, c;
-                sincospif((float)(2.0 * turns), &s, &c);
+                sincos_turns<T>(pos * p.freqs[pr], s, c);
                 cs[j] = c * p.factor;
                 sn[j] = s * p.factor * p.sign;
             }
@@ -151,10 +163,11 @@ cudaError_t launch(RotaryParams p, const void* q, const void* k, void* qo, void*
     const int slots = PAIRED ? p.pairs / V + (p.dim - 2 * p.pairs) / V : p.dim / V;
     const int64_t n = (int64_t)p.batch * p.len * slots;
     const int heads = p.hq + p.hk;
-    // Few tokens: spread the heads over threads too (a thread that walks 32 heads in a row waits for
-    // memory eight times); many tokens: one thread does all heads of its slot and forms the sines once.
+    // Few tokens: spread the heads over threads too (a thread that walks 32 heads in a row waits for memory eight
+    // times); otherwise one thread does all heads of its slot, since the way to its sines (position, frequency, 64-bit
+    // product) is a fixed latency: 40 heads of 128 at 16384 tokens 61 us, halved 64, in quarters 70.
     int per = heads;
-    while (per > 4 && n * ((heads + per - 1) / per) < 148LL * 1024) per = (per + 1) / 2;
+    while (per > 4 && n * ((heads + per - 1) / per) < 148LL * 512) per = (per + 1) / 2;
     p.heads_per_thread = per;
     const int threads = 256;
     const int64_t blocks = (n + threads - 1) / threads;
