@@ -968,23 +968,39 @@ int np_of(int N) { return 4 * ns_of(N); }
 int tok_of(int N) { return ns_of(N) >= 8 ? 16 : 32; }
 int tiles_per_group(const ScanParams& p) { return (p.channels / p.groups + kCB - 1) / kCB; }
 
-// One CTA walks a whole sequence unless that leaves SMs without work: then the tokens are cut so that
-// about two CTAs per SM exist.  A segment is at least four tiles: its local pass and the combination of the
-// segments before it have to stay small beside it.
-void cut(ScanParams& p) {
+// One CTA walks a whole sequence unless that leaves SMs without work: with fewer CTAs than SMs the tokens are cut
+// into segments, as many as fill the places for CTAs (three per SM forward, two backward: registers) in one round, or
+// in two or three where that leaves fewer of them empty.  B1-T8192-C4096 forward, 64 CTAs: 3 segments 711 us, 6 (one
+// round, 86 %) 562, 7 (a second round of four CTAs) 587, 13 (two rounds, 94 %) 519; B1-T16384-C1024 backward, 16 CTAs:
+// 9 segments 962 us, 18 (97 %) 626, 23 823.  Not from 148 CTAs on: the local pass costs more than half of the main
+// one (8 rows of 2048 channels, 256 CTAs, forward: 1 segment 701 us, 2 segments 1028).
+// A segment is at least four tiles: its local pass and the combination of the segments before it have to stay small.
+void cut(ScanParams& p, bool backward) {
     const int tok = tok_of(p.states);
     const int64_t ctas = (int64_t)p.batch * p.groups * tiles_per_group(p), tiles = (p.len + tok - 1) / tok;
-    int64_t segs = ctas > 0 ? (2 * 148 + ctas - 1) / ctas : 1;
+    const int64_t places = 148 * (backward ? 2 : 3);
+    int64_t segs = 1;
+    if (ctas > 0 && ctas < 148) {
+        double fullest = 0.0;
+        for (int64_t rounds = 1; rounds <= 3 && fullest < 0.93; ++rounds) {
+            const int64_t n = places * rounds / ctas;
+            const double full = (double)(n * ctas) / (double)(places * rounds);
+            if (n >= 1 && full > fullest + 0.02) {
+                fullest = full;
+                segs = n;
+            }
+        }
+    }
     if (segs > tiles / 4) segs = tiles / 4;
-    if (segs < 1 || ctas >= 148) segs = 1;
-    const int64_t per = segs > 0 ? (tiles + segs - 1) / segs : 1;
+    if (segs < 1) segs = 1;
+    const int64_t per = (tiles + segs - 1) / segs;
     p.seg_len = (per > 0 ? per : 1) * tok;
     p.segs = p.len > 0 ? (int)((p.len + p.seg_len - 1) / p.seg_len) : 1;
 }
 
 int64_t seg_floats(const ScanParams& p) { return p.segs > 1 ? (int64_t)p.batch * p.segs * p.channels * (np_of(p.states) + 1) : 0; }
 
-int resolve(const fbla_scan_problem* p, ScanParams* r) {
+int resolve(const fbla_scan_problem* p, bool backward, ScanParams* r) {
     using fbla::api_fail;
     if (p == nullptr) return api_fail(FBLA_ERR_INVALID, "problem is NULL");
     if (p->dtype != FBLA_F32 && p->dtype != FBLA_BF16 && p->dtype != FBLA_F16)
@@ -1018,7 +1034,7 @@ int resolve(const fbla_scan_problem* p, ScanParams* r) {
     r->cu = p->cu_seqlens;
     r->A = r->D = r->bias = nullptr;
     r->vec = 0;
-    cut(*r);
+    cut(*r, backward);
     return FBLA_OK;
 }
 
@@ -1171,14 +1187,14 @@ extern "C" {
 
 int64_t fbla_selective_scan_checkpoint_floats(const fbla_scan_problem* p) {
     ScanParams r;
-    if (resolve(p, &r) != FBLA_OK) return -1;
+    if (resolve(p, false, &r) != FBLA_OK) return -1;
     const int tok = tok_of(r.states);
     return (int64_t)r.batch * ((r.len + tok - 1) / tok) * r.channels * np_of(r.states);
 }
 
 int64_t fbla_selective_scan_workspace_bytes(const fbla_scan_problem* p, int backward) {
     ScanParams r;
-    if (resolve(p, &r) != FBLA_OK) return -1;
+    if (resolve(p, backward != 0, &r) != FBLA_OK) return -1;
     return (backward ? bwd_layout(r).total : seg_floats(r)) * (int64_t)sizeof(float);
 }
 
@@ -1187,7 +1203,7 @@ int fbla_selective_scan_fwd(const fbla_scan_problem* p, const void* x, const voi
                             float* checkpoints, void* workspace, size_t workspace_bytes, fbla_stream_t stream) {
     using fbla::api_fail;
     ScanParams r;
-    if (int rc = resolve(p, &r)) return rc;
+    if (int rc = resolve(p, false, &r)) return rc;
     if (A == nullptr) return api_fail(FBLA_ERR_INVALID, "A is NULL");
     if (r.batch > 0 && r.len > 0 && (x == nullptr || dt == nullptr || B == nullptr || C == nullptr || y == nullptr))
         return api_fail(FBLA_ERR_INVALID, "x, dt, B, C or y is NULL");
@@ -1214,7 +1230,7 @@ int fbla_selective_scan_bwd(const fbla_scan_problem* p, const void* x, const voi
                             fbla_stream_t stream) {
     using fbla::api_fail;
     ScanParams r;
-    if (int rc = resolve(p, &r)) return rc;
+    if (int rc = resolve(p, true, &r)) return rc;
     if (A == nullptr || dA == nullptr) return api_fail(FBLA_ERR_INVALID, "A or dA is NULL");
     if (r.batch > 0 && r.len > 0 && (x == nullptr || dt == nullptr || B == nullptr || C == nullptr || dy == nullptr || dx == nullptr ||
                                      ddt == nullptr || dB == nullptr || dC == nullptr || checkpoints == nullptr))
@@ -1241,7 +1257,7 @@ int fbla_selective_scan_step(const fbla_scan_problem* p, const void* x, const vo
                              const float* D, const void* z, const float* dt_bias, float* state, void* y, fbla_stream_t stream) {
     using fbla::api_fail;
     ScanParams r;
-    if (int rc = resolve(p, &r)) return rc;
+    if (int rc = resolve(p, false, &r)) return rc;
     if (r.cu != nullptr) return api_fail(FBLA_ERR_INVALID, "cu_seqlens given to the single-token step");
     if (r.batch == 0) return FBLA_OK;
     if (x == nullptr || dt == nullptr || A == nullptr || B == nullptr || C == nullptr || state == nullptr || y == nullptr)
