@@ -90,49 +90,83 @@ template <int NS> struct States {
 #pragma unroll
         for (int i = 0; i < NS / 2; ++i) v[i] = F2(0.f);
     }
-    __device__ __forceinline__ void load(const float* p) {      // aligned to 4 * NS bytes
+    // NS floats at p, aligned to 4 * NS bytes.  With `swap` the two halves change places (see sum_channels).
+    __device__ __forceinline__ void load(const float* p, bool swap = false) {
+        if constexpr (NS == 2) {
+            v[0].v = *reinterpret_cast<const unsigned long long*>(p);
+        } else {
+            const float *lo = p + (swap ? NS / 2 : 0), *hi = p + (swap ? 0 : NS / 2);
 #pragma unroll
-        for (int i = 0; i < NS / 4; ++i) {
-            const ulonglong2 w = reinterpret_cast<const ulonglong2*>(p)[i];
-            v[2 * i].v = w.x;
-            v[2 * i + 1].v = w.y;
+            for (int i = 0; i < NS / 4; ++i) {
+                v[i].v = reinterpret_cast<const unsigned long long*>(lo)[i];
+                v[NS / 4 + i].v = reinterpret_cast<const unsigned long long*>(hi)[i];
+            }
         }
-        if (NS == 2) v[0].v = *reinterpret_cast<const unsigned long long*>(p);
     }
-    __device__ __forceinline__ void store(float* p) const {
+    __device__ __forceinline__ void store(float* p, bool swap = false) const {
+        if constexpr (NS == 2) {
+            *reinterpret_cast<unsigned long long*>(p) = v[0].v;
+        } else {
+            float *lo = p + (swap ? NS / 2 : 0), *hi = p + (swap ? 0 : NS / 2);
 #pragma unroll
-        for (int i = 0; i < NS / 4; ++i) reinterpret_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i].v, v[2 * i + 1].v);
-        if (NS == 2) *reinterpret_cast<unsigned long long*>(p) = v[0].v;
+            for (int i = 0; i < NS / 4; ++i) {
+                reinterpret_cast<unsigned long long*>(lo)[i] = v[i].v;
+                reinterpret_cast<unsigned long long*>(hi)[i] = v[NS / 4 + i].v;
+            }
+        }
+    }
+    // The same in one piece, of 16 bytes where there are as many
+    __device__ __forceinline__ void load_wide(const float* p) {
+        if constexpr (NS == 2) {
+            load(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS / 4; ++i) {
+                const ulonglong2 w = reinterpret_cast<const ulonglong2*>(p)[i];
+                v[2 * i].v = w.x;
+                v[2 * i + 1].v = w.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void store_wide(float* p) const {
+        if constexpr (NS == 2) {
+            store(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS / 4; ++i) reinterpret_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i].v, v[2 * i + 1].v);
+        }
     }
     // A caller's (.., channels, N) tensor; the states behind N are zero.
-    __device__ __forceinline__ void load_user(const float* row, int n0, int N) {
+    __device__ __forceinline__ void load_user(const float* row, int n0, int N, bool swap) {
         if (N == 4 * NS) {
-            load(row + n0);
+            load(row + n0, swap);
         } else {
 #pragma unroll
             for (int i = 0; i < NS / 2; ++i) {
-                const int n = n0 + 2 * i;
+                const int n = n0 + (swap && NS > 2 ? (2 * i) ^ (NS / 2) : 2 * i);
                 v[i] = F2(n < N ? row[n] : 0.f, n + 1 < N ? row[n + 1] : 0.f);
             }
         }
     }
-    __device__ __forceinline__ void store_user(float* row, int n0, int N) const {
+    __device__ __forceinline__ void store_user(float* row, int n0, int N, bool swap) const {
         if (N == 4 * NS) {
-            store(row + n0);
+            store(row + n0, swap);
         } else {
 #pragma unroll
             for (int i = 0; i < NS / 2; ++i) {
-                const int n = n0 + 2 * i;
+                const int n = n0 + (swap && NS > 2 ? (2 * i) ^ (NS / 2) : 2 * i);
                 if (n < N) row[n] = v[i].x();
                 if (n + 1 < N) row[n + 1] = v[i].y();
             }
         }
     }
-    __device__ __forceinline__ float sum() const {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < NS / 2; ++i) s += v[i].x() + v[i].y();
-        return s;
+    __device__ __forceinline__ void load_user(const float* row, int n0, int N) {
+        if (N == 4 * NS) load_wide(row + n0);
+        else load_user(row, n0, N, false);
+    }
+    __device__ __forceinline__ void store_user(float* row, int n0, int N) const {
+        if (N == 4 * NS) store_wide(row + n0);
+        else store_user(row, n0, N, false);
     }
 };
 
@@ -145,7 +179,8 @@ template <int NS> struct Place {
     int warp, lane, q;          // q: which states the lane holds
     int slot, c;                // the lane's two channels: their slot in a row of shared memory, the number of the first
     bool live[2];
-    __device__ __forceinline__ Place(const ScanParams& p) {
+    bool swap;                  // the lane holds the halves of its states the other way round (backward pass)
+    __device__ __forceinline__ explicit Place(const ScanParams& p, bool exchange = false) {
         const int cpg = p.channels / p.groups, tpg = (cpg + kCB - 1) / kCB;
         b = blockIdx.z;
         seg = blockIdx.y;
@@ -160,6 +195,7 @@ template <int NS> struct Place {
         c = c0 + (slot % L::kTPR) * L::kVPT + slot / L::kTPR * 2;
         live[0] = c < cend;
         live[1] = c + 1 < cend;
+        swap = exchange && (lane & 16) != 0;
     }
     // When a tile is loaded or stored a thread has kVPT consecutive channels of one token; the channels 2 i and
     // 2 i + 1 of them lie at slot(i): threads next to each other write next to each other, and so read the lanes
@@ -201,7 +237,7 @@ __device__ __forceinline__ States<NS> state_before(const ScanParams& p, const Pl
         const int f = m.first[tt];
         if (f >= 0) {
             r.zero();
-            if (init != nullptr && at.live[ch]) r.load_user(init + ((int64_t)f * p.channels + at.c + ch) * p.states, at.q * NS, p.states);
+            if (init != nullptr && at.live[ch]) r.load_user(init + ((int64_t)f * p.channels + at.c + ch) * p.states, at.q * NS, p.states, at.swap);
         }
     }
     return r;
@@ -246,11 +282,14 @@ template <typename T, int NS> struct BCShare {
             v[k] = n < p.states && t0 + t < end ? base[(t0 + t) * st[1] + n] : from_f<T>(0.f);
         }
     }
-    template <bool VARLEN> __device__ __forceinline__ void put(float* dst, const Marks& m) const {
+    // `swapped`: a second copy with the halves of each lane's states exchanged
+    template <bool VARLEN> __device__ __forceinline__ void put(float* dst, const Marks& m, float* swapped = nullptr) const {
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             const int i = threadIdx.x + k * kThreads;
-            dst[i] = !VARLEN || m.inside[i / L::kNP] ? to_f<T>(v[k]) : 0.f;
+            const float x = !VARLEN || m.inside[i / L::kNP] ? to_f<T>(v[k]) : 0.f;
+            dst[i] = x;
+            if (swapped != nullptr) swapped[i ^ (NS / 2)] = x;
         }
     }
 };
@@ -274,7 +313,7 @@ template <int NS> __device__ __forceinline__ void load_rates(const ScanParams& p
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
         A2[ch].zero();
-        if (at.live[ch]) A2[ch].load_user(p.A + (int64_t)(at.c + ch) * p.states, at.q * NS, p.states);
+        if (at.live[ch]) A2[ch].load_user(p.A + (int64_t)(at.c + ch) * p.states, at.q * NS, p.states, at.swap);
 #pragma unroll
         for (int i = 0; i < NS / 2; ++i) A2[ch].v[i] = mul2(A2[ch].v[i], F2(1.44269504f));
     }
@@ -295,7 +334,7 @@ __device__ __forceinline__ void add_segment(const ScanParams& p, const Place<NS>
         const int64_t k = seg_at<NS>(p, at.b, j, at.c + ch);
         const float sd = seg_d[k];
         States<NS> own;
-        own.load(seg_v + k * Tile<NS>::kNP + at.q * NS);
+        own.load(seg_v + k * Tile<NS>::kNP + at.q * NS, at.swap);
 #pragma unroll
         for (int i = 0; i < NS / 2; ++i)
             v[ch].v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2[ch].v[i])), v[ch].v[i], own.v[i]);
@@ -395,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch)
                 if (ckpt != nullptr && at.live[ch])
-                    h[ch].store(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0));
+                    h[ch].store_wide(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0));
         }
 #pragma unroll 1
         for (int tt = 0; tt < L::kTok; tt += 4) {
@@ -404,8 +443,8 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
             for (int k = 0; k < 4; ++k) {
                 const float4 v = sm.dx[tt + k][at.slot];
                 States<NS> Bv, Cv;
-                Bv.load(sm.B + (tt + k) * L::kNP + n0);
-                if (!LOCAL) Cv.load(sm.C + (tt + k) * L::kNP + n0);
+                Bv.load_wide(sm.B + (tt + k) * L::kNP + n0);
+                if (!LOCAL) Cv.load_wide(sm.C + (tt + k) * L::kNP + n0);
 #pragma unroll
                 for (int ch = 0; ch < 2; ++ch) {
                     const float d = ch ? v.z : v.x;
@@ -590,29 +629,48 @@ __global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanP
     }
 }
 
-// Sums over the eight channels of a warp (lane bits 2, 3, 4) of the M values each lane holds: halving
-// exchanges while there is something to halve.  Returns the index of the first value the lane ends with;
-// max(1, M / 8) of them are left in v[0 ..].
-template <int M> __device__ __forceinline__ int sum8(float (&v)[M], int lane) {
-    int first = 0, m = M;
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 shfl2(F2 a, int mask) {
+    return F2(__shfl_xor_sync(0xffffffffu, a.x(), mask), __shfl_xor_sync(0xffffffffu, a.y(), mask));
+}
+__device__ __forceinline__ F2 pick(bool first, F2 a, F2 b) { return F2(first ? a.x() : b.x(), first ? a.y() : b.y()); }
+
+// Sums of dB and dC over the channels of a warp (lane bits 4, 3 and 2), by exchanges that halve what a lane holds:
+// first the halves of its states -- lanes with bit 4 hold them the other way round, so that every lane gives away its
+// second half and nothing has to be selected --, then dB against dC, then one of two pairs (of two values with four
+// states).  out: what is left, for consecutive columns of [dB | dC] from the returned one on.
+template <int NS> __device__ __forceinline__ int sum_channels(const F2 (&dB)[NS / 2], const F2 (&dC)[NS / 2], int lane, float (&out)[NS >= 8 ? 2 : 1]) {
+    const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
+    const int n0 = (lane & 3) * NS;
+    if constexpr (NS == 2) {
+        F2 v = add2(pick(!b4, dB[0], dC[0]), shfl2(pick(b4, dB[0], dC[0]), 16));
+        const float give = b3 ? v.x() : v.y(), keep = b3 ? v.y() : v.x();
+        out[0] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+        out[0] += __shfl_xor_sync(0xffffffffu, out[0], 4);
+        return (b4 ? Tile<NS>::kNP : 0) + n0 + (b3 ? 1 : 0);
+    } else {
+        constexpr int H = NS / 4;
+        F2 v[H];
 #pragma unroll
-    for (int mask = 16; mask >= 4; mask >>= 1) {
-        const bool up = lane & mask;
-        if (m > 1) {
-            m >>= 1;
-#pragma unroll
-            for (int i = 0; i < M / 2; ++i) {
-                if (i < m) {
-                    const float give = up ? v[i] : v[i + m], keep = up ? v[i + m] : v[i];
-                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, mask);
-                }
-            }
-            if (up) first += m;
+        for (int i = 0; i < H; ++i) {
+            const F2 b = add2(dB[i], shfl2(dB[H + i], 16)), c = add2(dC[i], shfl2(dC[H + i], 16));
+            v[i] = add2(pick(!b3, b, c), shfl2(pick(b3, b, c), 8));
+        }
+        const int col = (b3 ? Tile<NS>::kNP : 0) + n0 + (b4 ? NS / 2 : 0);
+        if constexpr (NS == 4) {
+            const float give = b2 ? v[0].x() : v[0].y(), keep = b2 ? v[0].y() : v[0].x();
+            out[0] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+            return col + (b2 ? 1 : 0);
         } else {
-            v[0] += __shfl_xor_sync(0xffffffffu, v[0], mask);
+            const F2 r = add2(pick(!b2, v[0], v[1]), shfl2(pick(b2, v[0], v[1]), 4));
+            r.get(out[0], out[1]);
+            return col + (b2 ? 2 : 0);
         }
     }
-    return first;
 }
 
 template <int NS> struct BwdSmem {
@@ -623,13 +681,15 @@ template <int NS> struct BwdSmem {
     float2 slope[L::kTok][kRow2];                   // dy silu'(z)
     float2 y[L::kTok][kRow2];                       // s = sum C h
     float2 gB[L::kTok][kRow2];                      // sum G B
-    float B[L::kTok * L::kNP], C[L::kTok * L::kNP];
+    float B[2][L::kTok * L::kNP], C[2][L::kTok * L::kNP];       // the second with the halves of the states exchanged
     float start[kSubs][2][kThreads][NS];            // each thread's states at the starts of the sub-tiles
     float dbc[kWarps][L::kTok][2 * L::kNP];         // per warp: sums of dB, dC over its channels
     float4 acc[L::kVPT / 2][kThreads];              // each thread's sums for dD (two channels) and dbias
     float2 D[kCB / 2], bias[kCB / 2];
     Marks marks;
 };
+
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // All gradients of one segment, tile after tile from its end.  In a tile the states are formed again from the
 // checkpoint, first up to the starts of its sub-tiles; then sub-tile after sub-tile, from the last one, with
@@ -647,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     constexpr int K = L::kSub, V = L::kVPT, P = NS / 2;
     extern __shared__ __align__(16) unsigned char raw_smem[];
     BwdSmem<NS>& sm = *reinterpret_cast<BwdSmem<NS>*>(raw_smem);
-    const Place<NS> at(p);
+    const Place<NS> at(p, NS > 2);
     const int N = p.states, n0 = at.q * NS;
     const int64_t t0 = at.seg * p.seg_len, t1 = min(p.len, t0 + p.seg_len);
     const int64_t ntiles = (p.len + L::kTok - 1) / L::kTok;
@@ -660,10 +720,11 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         g[ch].zero();
         dA[ch].zero();
         if (!VARLEN && dfin != nullptr && at.live[ch] && at.seg == p.segs - 1)
-            g[ch].load_user(dfin + (at.b * p.channels + at.c + ch) * N, n0, N);
+            g[ch].load_user(dfin + (at.b * p.channels + at.c + ch) * N, n0, N, at.swap);
     }
     for (int j = p.segs - 1; j > at.seg; --j) add_segment<NS>(p, at, j, seg_g, seg_d, A2, g);
     const int row = at.row(), c = at.c0 + at.col();
+    const float *sB = sm.B[at.swap] + n0, *sC = sm.C[at.swap] + n0;     // the lane's states of token 0
     load_per_channel<NS>(p, at, p.D, sm.D);
     load_per_channel<NS>(p, at, p.bias, sm.bias);
 #pragma unroll
@@ -682,16 +743,16 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
             h[ch].zero();
-            if (at.live[ch]) h[ch].load(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0));
+            if (at.live[ch]) h[ch].load(ckpt + (((at.b * ntiles + tb / L::kTok) * p.channels + at.c + ch) * L::kNP + n0), at.swap);
         }
         {
             BwdShare<T, NS> in;
             if (ok) in.load(p, at, x, dt, z, dy, t);
             BCShare<T, NS> bc;
             bc.load(Bm, p.bs, p, at, tb, t1);
-            bc.template put<VARLEN>(sm.B, sm.marks);
+            bc.template put<VARLEN>(sm.B[0], sm.marks, NS > 2 ? sm.B[1] : nullptr);
             bc.load(Cm, p.cs, p, at, tb, t1);
-            bc.template put<VARLEN>(sm.C, sm.marks);
+            bc.template put<VARLEN>(sm.C[0], sm.marks, NS > 2 ? sm.C[1] : nullptr);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
                 const int s = at.slot_of(i);
@@ -714,18 +775,27 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             }
         }
         __syncthreads();
+        if (tb > t0) {                  // the tile before this one, on its way to L2
+            const int64_t u = t - L::kTok;
+            if (c < at.cend) {
+                prefetch(x + at.b * p.xs[0] + u * p.xs[1] + c);
+                prefetch(dt + at.b * p.ds[0] + u * p.ds[1] + c);
+                prefetch(dy + at.b * p.gs[0] + u * p.gs[1] + c);
+                if (z != nullptr) prefetch(z + at.b * p.zs[0] + u * p.zs[1] + c);
+            }
+        }
 
 #pragma unroll 1
         for (int sub = 0; sub < BwdSmem<NS>::kSubs; ++sub) {
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) h[ch].store(sm.start[sub][ch][threadIdx.x]);
+            for (int ch = 0; ch < 2; ++ch) h[ch].store_wide(sm.start[sub][ch][threadIdx.x]);
             if (sub == BwdSmem<NS>::kSubs - 1) break;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int tt = sub * K + k;
                 const float4 v = sm.dx[tt][at.slot];
                 States<NS> Bv;
-                Bv.load(sm.B + tt * L::kNP + n0);
+                Bv.load_wide(sB + tt * L::kNP);
 #pragma unroll
                 for (int ch = 0; ch < 2; ++ch) {
                     const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y);
@@ -739,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         for (int sub = BwdSmem<NS>::kSubs - 1; sub >= 0; --sub) {
             States<NS> a[2][K], hs[2][K + 1];
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) hs[ch][0].load(sm.start[sub][ch][threadIdx.x]);
+            for (int ch = 0; ch < 2; ++ch) hs[ch][0].load_wide(sm.start[sub][ch][threadIdx.x]);
 #pragma unroll
             for (int k0 = 0; k0 < K; k0 += 4) {
                 float ys[2][4];
@@ -748,8 +818,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                     const int tt = sub * K + k;
                     const float4 v = sm.dx[tt][at.slot];
                     States<NS> Bv, Cv;
-                    Bv.load(sm.B + tt * L::kNP + n0);
-                    Cv.load(sm.C + tt * L::kNP + n0);
+                    Bv.load_wide(sB + tt * L::kNP);
+                    Cv.load_wide(sC + tt * L::kNP);
 #pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
                         const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y);
@@ -776,15 +846,15 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                     const float4 v = sm.dx[tt][at.slot];
                     const float2 e = sm.e[tt][at.slot];
                     States<NS> Bv, Cv;
-                    Bv.load(sm.B + tt * L::kNP + n0);
-                    Cv.load(sm.C + tt * L::kNP + n0);
+                    Bv.load_wide(sB + tt * L::kNP);
+                    Cv.load_wide(sC + tt * L::kNP);
                     F2 dB[P], dC[P];
 #pragma unroll
                     for (int ch = 0; ch < 2; ++ch) {
                         const F2 d2(ch ? v.z : v.x), dx2(ch ? v.w : v.y), e2(ch ? e.y : e.x);
                         if (VARLEN && dfin != nullptr) {
                             const int l = sm.marks.last[tt];
-                            if (l >= 0 && at.live[ch]) g[ch].load_user(dfin + ((int64_t)l * p.channels + at.c + ch) * N, n0, N);
+                            if (l >= 0 && at.live[ch]) g[ch].load_user(dfin + ((int64_t)l * p.channels + at.c + ch) * N, n0, N, at.swap);
                         }
                         const States<NS> hp = state_before<NS, VARLEN>(p, at, sm.marks, tt, init, hs[ch][k], ch);
                         F2 gb2(0.f), ra2(0.f);
@@ -804,24 +874,15 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                         if (VARLEN) {
                             const int f = sm.marks.first[tt];
                             if (f >= 0) {
-                                if (dinit != nullptr && at.live[ch]) g[ch].store_user(dinit + ((int64_t)f * p.channels + at.c + ch) * N, n0, N);
+                                if (dinit != nullptr && at.live[ch]) g[ch].store_user(dinit + ((int64_t)f * p.channels + at.c + ch) * N, n0, N, at.swap);
                                 g[ch].zero();
                             }
                         }
                     }
-                    float bc[2 * NS];
-#pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        dB[i].get(bc[2 * i], bc[2 * i + 1]);
-                        dC[i].get(bc[NS + 2 * i], bc[NS + 2 * i + 1]);
-                    }
-                    const int first = sum8<2 * NS>(bc, at.lane);
-                    constexpr int LEFT = 2 * NS >= 8 ? 2 * NS / 8 : 1;
-#pragma unroll
-                    for (int i = 0; i < LEFT; ++i) {
-                        const int w = first + i;            // dB of state n0 + w, or dC of state n0 + w - NS
-                        sm.dbc[at.warp][tt][(w < NS ? n0 + w : L::kNP + n0 + w - NS)] = bc[i];
-                    }
+                    float sums[NS >= 8 ? 2 : 1];
+                    const int col = sum_channels<NS>(dB, dC, at.lane, sums);
+                    if constexpr (NS >= 8) *reinterpret_cast<float2*>(&sm.dbc[at.warp][tt][col]) = make_float2(sums[0], sums[1]);
+                    else sm.dbc[at.warp][tt][col] = sums[0];
                 }
                 const float g0 = sum4(gb[0], at.q), g1 = sum4(gb[1], at.q), r0 = sum4(ra[0], at.q), r1 = sum4(ra[1], at.q);
                 __syncwarp();               // the four lanes of a channel are done with its d x of these tokens
@@ -895,8 +956,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
         if (!at.live[ch]) continue;
-        dA[ch].store_user(part_A + (bs * p.channels + at.c + ch) * N, n0, N);
-        if (!VARLEN && dinit != nullptr && at.seg == 0) g[ch].store_user(dinit + (at.b * p.channels + at.c + ch) * N, n0, N);
+        dA[ch].store_user(part_A + (bs * p.channels + at.c + ch) * N, n0, N, at.swap);
+        if (!VARLEN && dinit != nullptr && at.seg == 0) g[ch].store_user(dinit + (at.b * p.channels + at.c + ch) * N, n0, N, at.swap);
     }
 }
 
