@@ -603,7 +603,10 @@ cudaError_t run_fwd(const ConvParams& p, const T* x, const T* init, T* y, T* fin
     constexpr int V = 4;
     const void* ptrs[3] = {x, init, y};
     if (p.len > 0 && p.batch > 0) {
-        const cudaError_t e = vec_ok(p, V, sizeof(T), ptrs, 3) ? launch_fwd<T, W, V>(p, x, init, y, st) : launch_fwd<T, W, 1>(p, x, init, y, st);
+        cudaError_t e;
+        if (vec_ok(p, V, sizeof(T), ptrs, 3)) e = launch_fwd<T, W, V>(p, x, init, y, st);
+        else if (vec_ok(p, 2, sizeof(T), ptrs, 3)) e = launch_fwd<T, W, 2>(p, x, init, y, st);
+        else e = launch_fwd<T, W, 1>(p, x, init, y, st);
         if (e != cudaSuccess) return e;
     }
     if (fin != nullptr && p.num_seqs > 0) {
@@ -636,10 +639,12 @@ cudaError_t run_bwd(const ConvParams& p, const T* x, const T* init, const T* dy,
     const void* ptrs[5] = {x, init, dy, dfin, dx};
     int64_t rows = 0;
     if (p.len > 0 && p.batch > 0) {
-        const bool vec = vec_ok(p, V, sizeof(T), ptrs, 5);
-        const cudaError_t e = vec ? launch_bwd<T, W, V>(p, x, init, dy, dfin, dx, ws, st) : launch_bwd<T, W, 1>(p, x, init, dy, dfin, dx, ws, st);
+        const int v = vec_ok(p, V, sizeof(T), ptrs, 5) ? V : vec_ok(p, 2, sizeof(T), ptrs, 5) ? 2 : 1;
+        const cudaError_t e = v == V ? launch_bwd<T, W, V>(p, x, init, dy, dfin, dx, ws, st)
+                            : v == 2 ? launch_bwd<T, W, 2>(p, x, init, dy, dfin, dx, ws, st)
+                                     : launch_bwd<T, W, 1>(p, x, init, dy, dfin, dx, ws, st);
         if (e != cudaSuccess) return e;
-        rows = shape_of(p, vec ? V : 1).blocks_t * p.batch;
+        rows = shape_of(p, v).blocks_t * p.batch;
     }
     const unsigned blocks = (unsigned)(((int64_t)p.channels * (W + 1) + 31) / 32);
     if (p.w32) conv_weight_grad_kernel<W, float><<<blocks, dim3(32, 8), 0, st>>>(ws, rows, p.channels, (float*)dw, (float*)db);
@@ -684,10 +689,12 @@ extern "C" {
 int64_t fbla_causal_conv_workspace_bytes(const fbla_conv_problem* p) {
     ConvParams r;
     if (resolve(p, &r) != FBLA_OK) return -1;
-    // the scalar and the vector kernel cut the tokens differently: the larger of the two
-    const int v = p->dtype == FBLA_F32 ? bwd_v<float>() : bwd_v<__half>();
-    const int64_t a = shape_of(r, 1).blocks_t, b = shape_of(r, v).blocks_t;
-    return (a > b ? a : b) * r.batch * (p->width + 1) * (int64_t)r.channels * (int64_t)sizeof(float);
+    int64_t most = 0;           // kernels of different widths cut the tokens differently
+    for (int v = 1; v <= 4; v *= 2) {
+        const int64_t blocks = shape_of(r, v).blocks_t;
+        most = blocks > most ? blocks : most;
+    }
+    return most * r.batch * (p->width + 1) * (int64_t)r.channels * (int64_t)sizeof(float);
 }
 
 int fbla_causal_conv_fwd(const fbla_conv_problem* p, const void* x, const void* w, const void* bias, const void* initial_state,
