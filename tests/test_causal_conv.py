@@ -209,3 +209,30 @@ def test_old_infinities_stay_in_their_window():
     x[0, 3, 1] = float("inf")
     y = causal_conv1d(x.cuda(), torch.ones(4, 3).cuda()).cpu()
     assert y[0, 3:6, 1].isinf().all() and int(y.isfinite().logical_not().sum()) == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [22, 30, 257])
+@pytest.mark.parametrize("cu", [None, [0, 3, 70, 71]])
+def test_channel_counts_between_the_packs(dtype, C, cu):
+    """Two channels at a time, or one, in the fixed and the packed layout."""
+    rn = randn(C)
+    W, n = 4, 2 if cu is None else len(cu) - 1
+    lead = (2, 71) if cu is None else (71,)
+    x, w, b, dy = rn(*lead, C, dtype=dtype), rn(C, W, dtype=dtype), rn(C, dtype=dtype), rn(*lead, C, dtype=dtype)
+    init, df = rn(n, W - 1, C, dtype=dtype), rn(n, W - 1, C, dtype=dtype)
+    cu = None if cu is None else torch.tensor(cu, dtype=torch.int32)
+    compare(run(x, w, b, "silu", init, dy, df, cu), x, w, b, "silu", init, dy, df, cu)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^32 elements: the last tokens are what they are on their own, with the inputs before them as state."""
+    T, C, W = 2_200_000, 2048, 4
+    x = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(0))
+    w = torch.randn(C, W, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    y, end = causal_conv1d(x, w, activation="silu", return_final_state=True)
+    lo = T - 50
+    tail, end2 = causal_conv1d(x[:, lo:].clone(), w, activation="silu", initial_state=x[:, lo - W + 1:lo].clone(), return_final_state=True)
+    assert torch.equal(y[:, lo:], tail) and torch.equal(end, end2)

@@ -254,3 +254,13 @@ def test_one_gradient_alone_and_graph_capture():
     x.copy_(rn(2, 3, 10, 32))
     g.replay()
     assert torch.equal(out, rotary_embedding(x, None, fd))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    L, H, D = 1_050_000, 32, 128
+    q = torch.empty(1, L, H, D, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(0))
+    f = freqs_of(64).cuda()
+    got = rotary_embedding(q, None, f, layout="blhd")
+    tail = rotary_embedding(q[:, -40:].clone(), None, f, offset=L - 40, layout="blhd")
+    assert torch.equal(got[:, -40:], tail)

@@ -282,3 +282,33 @@ def test_same_bits_on_every_run_and_empty_inputs():
     e = {k: (v if k in ("A", "D", "bias") else v[:0]) for k, v in t.items()}
     got = run(e, dy[:0], df[:0], True)
     assert got["y"].shape == (0, 515, 72) and not got["dA"].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("C,G,N", [(23, 1, 16), (42, 2, 7), (136, 1, 16), (67, 1, 30)])
+@pytest.mark.parametrize("cu", [[0, 33, 33, 34, 200], [3, 64, 96, 640]])
+def test_packed_channel_counts(dtype, C, G, N, cu):
+    """Rows that start off boundaries, and boundaries of sequences on and inside tiles, with segments."""
+    T = cu[-1] + 2
+    t, dy, df = inputs(T + C, (T,), C, G, N, dtype, len(cu) - 1)
+    cu = torch.tensor(cu, dtype=torch.int32)
+    compare(run(t, dy, df, True, cu), t, dy, df, True, cu)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^32 elements: the last tokens are what they are on their own from the state before them."""
+    T, C, N = 1_050_000, 4096, 4
+    g = torch.Generator("cuda").manual_seed(0)
+    x = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    dt = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").uniform_(0.01, 0.2, generator=g)
+    Bm = torch.randn(1, T, N, device="cuda", generator=g).bfloat16()
+    A = -torch.rand(C, N, device="cuda", generator=g) - 0.5
+    y, end = selective_scan(x, dt, A, Bm, Bm, return_final_state=True)
+    lo = T - 64                         # exp(-0.5 * 0.1 * 5000) leaves nothing of what came before the last 5000 tokens
+    part = lambda v, a: v[:, a:].clone()                                # noqa: E731
+    tail, end2 = selective_scan(part(x, lo - 6000), part(dt, lo - 6000), A, part(Bm, lo - 6000), part(Bm, lo - 6000), return_final_state=True)
+    # sums of the same terms in other segments: 8 roundings for each of the 400 tokens that matter, of terms below 64
+    assert (y[:, lo:].float() - tail[:, -64:].float()).abs().max() <= 2.0 ** -8 * y[:, lo:].float().abs().max() + 3200 * 2.0 ** -24 * 64
+    assert (end - end2).abs().max() <= 3200 * 2.0 ** -24 * 64
