@@ -4,7 +4,8 @@
 other operators.  Timing: CUDA events around back-to-back calls of the public API, median of
 ``--reps`` repetitions after warm-up; inputs are larger than L2 from T=4096 up at B=8.
 
-    python benchmarks/benchmark_ops.py [--batch 8] [--op linear_attn|layers|fp32|blhd|simple_la|decoupled_la|varlen|pisa|all]
+    python benchmarks/benchmark_ops.py [--batch 8]
+                                       [--op linear_attn|layers|fp32|blhd|simple_la|decoupled_la|varlen|pisa|sequence|all]
                                        [--long] [--impl b200|reference [--ref-path DIR]]
 
 ``--long`` adds ``simple_la`` at B4 H32 T262144 D128 (8.6 GB per tensor, about 70 GB on the device).
@@ -191,6 +192,26 @@ def main():
         P = b * h * T * d * 2
         f, fb = both(lambda: piecewise_sparse_attention(q, k, v), (q, k, v), None if IMPL == "reference" else do)
         row("pisa", f"B{b} H{h} T{T} D{d} bs64 d0.1", f, fb, b * T, 7 * P, 7 * P)
+    if args.op in ("all", "sequence") and IMPL != "reference":
+        from flash_bla.ops.rotary.fused import rotary_embedding, rotary_frequencies
+        from flash_bla.ops.selective_scan.conv import causal_conv1d
+        from flash_bla.ops.selective_scan.scan import selective_scan
+        q = gau(B, H, 32768, D)
+        freqs, _ = rotary_frequencies(D)
+        P = q.numel() * 2
+        f, fb = both(lambda: rotary_embedding(q, None, freqs, interleaved=True), (q,), torch.randn_like(q))
+        row("rotary", f"B{B} H{H} T32768 D{D}", f, fb, B * 32768, 2 * P, 4 * P)
+        T, C, N = 4096, H * D * 2, 16
+        x, w, z, dt = gau(B, T, C), gau(C, 4), gau(B, T, C), gau(B, T, C)
+        Bm, Cm = gau(B, T, N), gau(B, T, N)
+        A = (-torch.arange(1.0, N + 1, device=dev).repeat(C, 1)).requires_grad_()
+        bias = torch.full((C,), -4.0, device=dev).requires_grad_()
+        do = torch.randn_like(x)
+        P = x.numel() * 2
+        f, fb = both(lambda: causal_conv1d(x, w, activation="silu"), (x, w), do)
+        row("causal_conv1d", f"B{B} T{T} C{C} W4", f, fb, B * T, 2 * P, 5 * P)
+        f, fb = both(lambda: selective_scan(x, dt, A, Bm, Cm, None, z, bias, dt_softplus=True), (x, dt, A, Bm, Cm, z, bias), do)
+        row("selective_scan", f"B{B} T{T} C{C} N{N}", f, fb, B * T, 4 * P, 11 * P)
 
 
 if __name__ == "__main__":
