@@ -20,34 +20,6 @@
 
 #include "seq_common.cuh"
 
-namespace fbla {
-namespace seq {
-
-namespace {
-template <typename OT>
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ in, int64_t rows, int64_t n, OT* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.f;
-    for (int64_t r = 0; r < rows; ++r) s += in[r * n + i];
-    out[i] = from_f<OT>(s);
-}
-}  // namespace
-
-cudaError_t sum_rows(const float* in, int64_t rows, int64_t n, int out_dtype, void* out, cudaStream_t st) {
-    if (n == 0) return cudaSuccess;
-    const int64_t blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    if (out_dtype == FBLA_F32) sum_rows_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(in, rows, n, (float*)out);
-    else if (out_dtype == FBLA_BF16) sum_rows_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(in, rows, n, (__nv_bfloat16*)out);
-    else sum_rows_kernel<__half><<<(unsigned)blocks, 256, 0, st>>>(in, rows, n, (__half*)out);
-    note_launches(1);
-    return cudaGetLastError();
-}
-
-}  // namespace seq
-}  // namespace fbla
-
 namespace {
 
 using fbla::from_f;

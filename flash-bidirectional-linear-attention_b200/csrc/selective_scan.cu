@@ -191,6 +191,10 @@ int fbla_selective_scan_step(const fbla_scan_problem* p, const void* x, const vo
     r.D = D;
     r.bias = dt_bias;
     r.segs = 1;
+    const int ns = ns_of(r.states), elem = p->dtype == FBLA_F32 ? 4 : 2;
+    r.vec = r.states == 4 * ns && fbla::seq::aligned_to(B, ns * elem > 16 ? 16 : ns * elem) &&
+            fbla::seq::aligned_to(C, ns * elem > 16 ? 16 : ns * elem);
+    for (int i = 0; i < 3; i += 2) r.vec = r.vec && r.bs[i] % ns == 0 && r.cs[i] % ns == 0;
     ScanTensors a = {};
     a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z; a.fin = state; a.y = y;
     return finish(with_type(p->dtype, [&](auto* t) { return Launcher<std::remove_pointer_t<decltype(t)>>::step(r, a, (cudaStream_t)stream); }),

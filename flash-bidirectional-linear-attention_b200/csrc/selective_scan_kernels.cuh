@@ -1034,18 +1034,48 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
     }
 }
 
-// dB, dC (batch, token, group, N) from the channel tiles' sums, tiles in order.
+// What follows the backward pass, in one launch: dB, dC (batch, token, group, N) from the channel tiles' sums, and dA, dD
+// and d_dt_bias from the segments', all in order.  The first `bc_blocks` blocks do the former.
+struct SumParams {
+    const float *bc, *A, *D, *bias;
+    float *dA, *dD, *dbias;
+    int64_t bc_rows, seg_rows, bc_blocks;
+    int tiles, channels, states;
+};
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) scan_bc_kernel(const float* __restrict__ part, int tiles, int64_t rows, int N, T* __restrict__ dB,
-                                                      T* __restrict__ dC) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= rows * 2 * NP) return;
-    const int64_t r = i / (2 * NP);
-    const int w = (int)(i % (2 * NP)), n = w % NP;
-    if (n >= N) return;
+__global__ void __launch_bounds__(256) scan_sums_kernel(const SumParams p, T* __restrict__ dB, T* __restrict__ dC) {
+    if ((int64_t)blockIdx.x < p.bc_blocks) {
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (i >= p.bc_rows * 2 * NP) return;
+        const int64_t r = i / (2 * NP);
+        const int w = (int)(i % (2 * NP)), n = w % NP;
+        if (n >= p.states) return;
+        float s = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < p.tiles; ++k) s += p.bc[k * p.bc_rows * 2 * NP + i];
+        (w < NP ? dB : dC)[r * p.states + n] = from_f<T>(s);
+        return;
+    }
+    const int64_t nA = (int64_t)p.channels * p.states, i = ((int64_t)blockIdx.x - p.bc_blocks) * 256 + threadIdx.x;
+    const float* in;
+    float* out;
+    int64_t n, at;
+    if (i < nA) {
+        in = p.A, out = p.dA, n = nA, at = i;
+    } else {
+        at = i - nA, n = p.channels;
+        if (at < n) {
+            in = p.D, out = p.dD;
+        } else {
+            at -= n;
+            in = p.bias, out = p.dbias;
+        }
+        if (at >= n || out == nullptr) return;
+    }
     float s = 0.f;
-    for (int k = 0; k < tiles; ++k) s += part[k * rows * 2 * NP + i];
-    (w < NP ? dB : dC)[r * N + n] = from_f<T>(s);
+#pragma unroll 4
+    for (int64_t r = 0; r < p.seg_rows; ++r) s += in[r * n + at];
+    out[at] = s;
 }
 
 // One token per row, the state updated in place.  Four lanes per channel: a state is read and written once, 16 bytes
@@ -1071,14 +1101,23 @@ __global__ void __launch_bounds__(4 * kStepChannels) scan_step_kernel(const Scan
         float d = to_f<T>(dt[b * p.ds[0] + c]);
         if (p.bias != nullptr) d += p.bias[c];
         if (p.softplus) d = fbla::seq::softplus(d);
+        Pack<T, NS> Bv, Cv;
+        if (p.vec) {                    // N is 4 NS and the rows of B and C start on boundaries
+            Bv.load(Bp + n0);
+            Cv.load(Cp + n0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                Bv.e[i] = n0 + i < N ? Bp[n0 + i] : from_f<T>(0.f);
+                Cv.e[i] = n0 + i < N ? Cp[n0 + i] : from_f<T>(0.f);
+            }
+        }
         F2 s2(0.f);
 #pragma unroll
         for (int i = 0; i < NS / 2; ++i) {
-            const int n = n0 + 2 * i;
-            const F2 Bv(n < N ? to_f<T>(Bp[n]) : 0.f, n + 1 < N ? to_f<T>(Bp[n + 1]) : 0.f);
-            const F2 Cv(n < N ? to_f<T>(Cp[n]) : 0.f, n + 1 < N ? to_f<T>(Cp[n + 1]) : 0.f);
-            h.v[i] = fma2(decay2(mul2(F2(d), mul2(A.v[i], F2(1.44269504f)))), h.v[i], mul2(F2(d * xv), Bv));
-            s2 = fma2(Cv, h.v[i], s2);
+            const F2 a = decay2(mul2(F2(d), mul2(A.v[i], F2(1.44269504f))));
+            h.v[i] = fma2(a, h.v[i], mul2(F2(d * xv), F2(Bv.get(2 * i), Bv.get(2 * i + 1))));
+            s2 = fma2(F2(Cv.get(2 * i), Cv.get(2 * i + 1)), h.v[i], s2);
         }
         acc = s2.x() + s2.y();
         h.store_user(hp, n0, N);
@@ -1186,16 +1225,25 @@ template <typename T, int NS, bool VARLEN, bool VEC> cudaError_t run_bwd(const S
                                                      a.ws + l.bc, a.ws + l.A, a.ws + l.D, a.ws + l.bias);
         fbla::note_launches(1);
         if (cudaError_t e = cudaGetLastError()) return e;
-        const int64_t tok = (int64_t)p.batch * p.len * p.groups, n = tok * 2 * Tile<NS>::kNP;
-        scan_bc_kernel<T, Tile<NS>::kNP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.ws + l.bc, tiles_per_group(p), tok, p.states,
-                                                                                     (T*)a.dB, (T*)a.dC);
-        fbla::note_launches(1);
     }
-    if (cudaError_t e = fbla::seq::sum_rows(a.ws + l.A, rows, (int64_t)p.channels * p.states, FBLA_F32, a.dA, st)) return e;
-    if (a.dD != nullptr)
-        if (cudaError_t e = fbla::seq::sum_rows(a.ws + l.D, rows, p.channels, FBLA_F32, a.dD, st)) return e;
-    if (a.dbias != nullptr)
-        if (cudaError_t e = fbla::seq::sum_rows(a.ws + l.bias, rows, p.channels, FBLA_F32, a.dbias, st)) return e;
+    SumParams q;
+    q.bc = a.ws + l.bc;
+    q.A = a.ws + l.A;
+    q.D = a.ws + l.D;
+    q.bias = a.ws + l.bias;
+    q.dA = a.dA;
+    q.dD = a.dD;
+    q.dbias = a.dbias;
+    q.bc_rows = any ? (int64_t)p.batch * p.len * p.groups : 0;
+    q.seg_rows = rows;
+    q.bc_blocks = (q.bc_rows * 2 * Tile<NS>::kNP + 255) / 256;
+    q.tiles = tiles_per_group(p);
+    q.channels = p.channels;
+    q.states = p.states;
+    const int64_t blocks = q.bc_blocks + ((int64_t)p.channels * (p.states + 2) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    scan_sums_kernel<T, Tile<NS>::kNP><<<(unsigned)blocks, 256, 0, st>>>(q, (T*)a.dB, (T*)a.dC);
+    fbla::note_launches(1);
     return cudaGetLastError();
 }
 

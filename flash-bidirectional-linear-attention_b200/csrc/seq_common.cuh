@@ -169,11 +169,6 @@ __device__ __forceinline__ SeqSpan seq_of(const int32_t* cu, int n, int64_t t) {
     return r;
 }
 
-// ---- sums over rows -------------------------------------------------------------------------------
-// out[i] = sum over r of in[r * n + i], rows in order: how per-block partial sums become one gradient
-// with the same bits on every run.
-cudaError_t sum_rows(const float* in, int64_t rows, int64_t n, int out_dtype, void* out, cudaStream_t st);
-
 inline bool aligned_to(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0; }
 
 }  // namespace seq
