@@ -38,9 +38,7 @@ def dense(t):
 
 def new(t):
     """A contiguous tensor of the shape, dtype and device of ``t``."""
-    if t is None:
-        return None
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def aligned(t):

@@ -105,7 +105,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.aligned(S.dense(dfinal))
         prob = _problem(x, dt, A, B, C, z, ctx.softplus, cu, dy)
-        dx, ddt, dA, dB, dC, dD, dz, dbias = (S.new(t) for t in (x, dt, A, B, C, D, z, dt_bias))
+        dx, ddt, dA, dB, dC, dD, dz, dbias = map(S.new, (x, dt, A, B, C, D, z, dt_bias))
         dstate = S.new(state) if ctx.needs_input_grad[8] else None
         L = _C.lib()
         ws, n = S.scratch(L.fbla_selective_scan_workspace_bytes(ctypes.byref(prob), 1), x)
