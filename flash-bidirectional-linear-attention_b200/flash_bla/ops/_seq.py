@@ -58,6 +58,12 @@ def refuse_grad(what, *tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
+def refuse_second_order(what):
+    """At the head of a backward pass: with ``create_graph=True`` its results would look like constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative: its backward pass cannot run with create_graph=True")
+
+
 def call(fn, prob, like, *args):
     """One library call on the current stream of ``like``'s device."""
     with _C.device_guard(like):

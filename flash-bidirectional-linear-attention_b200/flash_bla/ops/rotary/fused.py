@@ -9,7 +9,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flash_bla import _C
 from flash_bla.ops import _seq as S
@@ -122,8 +121,8 @@ class RotaryFunction(torch.autograd.Function):
         return _rotate(q, k, freqs, positions, offset, factor, interleaved, axes, dims, cu, False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk):
+        S.refuse_second_order("rotary_embedding")
         freqs, positions, cu = ctx.saved_tensors
         offset, factor, interleaved, axes, dims = ctx.args
         dq = dq if ctx.needs_input_grad[0] else None

@@ -9,7 +9,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flash_bla import _C
 from flash_bla.ops import _seq as S
@@ -65,8 +64,8 @@ class CausalConv1dFunction(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dfinal):
+        S.refuse_second_order("causal_conv1d")
         x, weight, bias, state, cu = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.dense(dfinal)

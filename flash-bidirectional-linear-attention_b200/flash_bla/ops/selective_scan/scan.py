@@ -11,7 +11,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flash_bla import _C
 from flash_bla.ops import _seq as S
@@ -99,8 +98,8 @@ class SelectiveScanFunction(torch.autograd.Function):
         return y, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dfinal):
+        S.refuse_second_order("selective_scan")
         x, dt, A, B, C, D, z, dt_bias, state, cu, ckpt = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.aligned(S.dense(dfinal))

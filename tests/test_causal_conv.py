@@ -236,3 +236,19 @@ def test_offsets_beyond_32_bits():
     lo = T - 50
     tail, end2 = causal_conv1d(x[:, lo:].clone(), w, activation="silu", initial_state=x[:, lo - W + 1:lo].clone(), return_final_state=True)
     assert torch.equal(y[:, lo:], tail) and torch.equal(end, end2)
+
+
+@gpu
+def test_many_short_sequences_and_no_token_at_all():
+    """Sequences shorter than the filter, many of them empty; then packed rows without a single token."""
+    g = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, 3, (700,), generator=g)
+    cu = torch.cat((torch.zeros(1, dtype=torch.long), lengths.cumsum(0))).int()
+    rn = randn(12)
+    T, C, n = int(cu[-1]), 12, 700
+    x, w, b, dy, init, df = rn(T, C), rn(C, 4), rn(C), rn(T, C), rn(n, 3, C), rn(n, 3, C)
+    compare(run(x, w, b, "silu", init, dy, df, cu), x, w, b, "silu", init, dy, df, cu)
+    none = torch.zeros(4, dtype=torch.int32)
+    got = run(x[:0], w, b, None, init[:3], dy[:0], df[:3], none)
+    assert got["y"].shape == (0, C) and torch.equal(got["final"].cpu(), init[:3]) and torch.equal(got["dinit"].cpu(), df[:3])
+    assert not got["dw"].any() and not got["db"].any()

@@ -312,3 +312,39 @@ def test_offsets_beyond_32_bits():
     # sums of the same terms in other segments: 8 roundings for each of the 400 tokens that matter, of terms below 64
     assert (y[:, lo:].float() - tail[:, -64:].float()).abs().max() <= 2.0 ** -8 * y[:, lo:].float().abs().max() + 3200 * 2.0 ** -24 * 64
     assert (end - end2).abs().max() <= 3200 * 2.0 ** -24 * 64
+
+
+@gpu
+def test_many_short_sequences_and_no_token_at_all():
+    g = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, 3, (500,), generator=g)
+    cu = torch.cat((torch.zeros(1, dtype=torch.long), lengths.cumsum(0))).int()
+    t, dy, df = inputs(12, (int(cu[-1]),), 12, 1, 16, torch.float32, 500)
+    compare(run(t, dy, df, True, cu), t, dy, df, True, cu)
+    none = torch.zeros(4, dtype=torch.int32)
+    e = {k: v if k in ("A", "D", "bias") else v[:3] if k == "init" else v[:0] for k, v in t.items()}
+    got = run(e, dy[:0], df[:3], True, none)
+    assert got["y"].shape == (0, 12) and torch.equal(got["final"].cpu(), t["init"][:3]) and torch.equal(got["dinit"].cpu(), df[:3])
+    assert not got["dA"].any() and not got["dD"].any() and not got["dbias"].any()
+
+
+@gpu
+def test_only_the_final_state_or_only_the_output_is_used():
+    """A gradient that reaches one of the two results alone."""
+    t, dy, df = inputs(13, (2, 40), 24, 1, 16, torch.float32, 2)
+    zero = torch.zeros_like
+    for use in ("y", "final"):
+        v = {k: leaf(x) for k, x in t.items()}
+        y, f = selective_scan(*(v[k] for k in NAMES[:8]), dt_softplus=True, initial_state=v["init"], return_final_state=True)
+        (y * dy.cuda()).sum().backward() if use == "y" else (f * df.cuda()).sum().backward()
+        got = dict(y=y, final=f, **{g: v[k].grad for k, g in zip(NAMES, GRADS)})
+        compare(got, t, dy if use == "y" else zero(dy), df if use == "final" else zero(df), True)
+
+
+@gpu
+def test_a_second_derivative_is_refused():
+    t, dy, _ = inputs(14, (1, 9), 8, 1, 4, torch.float32, 1)
+    v = {k: leaf(x) for k, x in t.items()}
+    y = selective_scan(*(v[k] for k in NAMES[:8]), dt_softplus=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y, v["x"], dy.cuda(), create_graph=True)
