@@ -75,7 +75,7 @@ int resolve(const fbla_scan_problem* p, bool backward, ScanParams* r) {
     }
     r->cu = p->cu_seqlens;
     r->A = r->D = r->bias = nullptr;
-    r->vec = 0;
+    r->vec = r->wide_A = 0;
     cut(*r, backward);
     return FBLA_OK;
 }
@@ -89,6 +89,12 @@ bool can_vec(const ScanParams& p, int elem, bool z, bool dy, std::initializer_li
     if (dy) ok = ok && p.gs[0] % v == 0 && p.gs[1] % v == 0;
     for (const void* q : ptrs) ok = ok && fbla::seq::aligned_to(q, bytes);
     return ok;
+}
+
+// A comes from a parameter and may lie anywhere, unlike the states: packs only where its address allows them.
+void set_rates(ScanParams& p, const float* A) {
+    p.A = A;
+    p.wide_A = p.states == np_of(p.states) && fbla::seq::aligned_to(A, 16);
 }
 
 template <typename F> cudaError_t with_type(int dtype, F f) {
@@ -139,7 +145,7 @@ int fbla_selective_scan_fwd(const fbla_scan_problem* p, const void* x, const voi
         return api_fail(FBLA_ERR_INVALID, "x, dt, B, C or y is NULL");
     if (int rc = check_ws(seg_floats(r) * (int64_t)sizeof(float), workspace, workspace_bytes)) return rc;
     if (int rc = check_states({initial_state, final_state, checkpoints, workspace})) return rc;
-    r.A = A;
+    set_rates(r, A);
     r.D = D;
     r.bias = dt_bias;
     r.vec = can_vec(r, p->dtype == FBLA_F32 ? 4 : 2, z != nullptr, false, {x, dt, z, y});
@@ -165,7 +171,7 @@ int fbla_selective_scan_bwd(const fbla_scan_problem* p, const void* x, const voi
     if ((z == nullptr) != (dz == nullptr)) return api_fail(FBLA_ERR_INVALID, "dz goes with z");
     if (int rc = check_ws(bwd_layout(r).total * (int64_t)sizeof(float), workspace, workspace_bytes)) return rc;
     if (int rc = check_states({initial_state, d_final_state, d_initial_state, checkpoints, workspace})) return rc;
-    r.A = A;
+    set_rates(r, A);
     r.D = D;
     r.bias = dt_bias;
     r.vec = can_vec(r, p->dtype == FBLA_F32 ? 4 : 2, z != nullptr, true, {x, dt, z, dy, dx, ddt, dz});
@@ -187,7 +193,7 @@ int fbla_selective_scan_step(const fbla_scan_problem* p, const void* x, const vo
     if (x == nullptr || dt == nullptr || A == nullptr || B == nullptr || C == nullptr || state == nullptr || y == nullptr)
         return api_fail(FBLA_ERR_INVALID, "x, dt, A, B, C, state or y is NULL");
     if (int rc = check_states({state})) return rc;
-    r.A = A;
+    set_rates(r, A);
     r.D = D;
     r.bias = dt_bias;
     r.segs = 1;

@@ -55,6 +55,7 @@ struct ScanParams {
     const int32_t* cu;
     const float *A, *D, *bias;
     int vec;                                // x, dt, z, dy, y can be read and written in packs
+    int wide_A;                             // A can be read in packs: no states behind N, and its address on a boundary
 };
 
 // Tokens of a tile: bounded by the shared memory that the sums over channels take in the backward pass.
@@ -140,9 +141,10 @@ template <int NS> struct States {
             for (int i = 0; i < NS / 4; ++i) reinterpret_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i].v, v[2 * i + 1].v);
         }
     }
-    // A caller's (.., channels, N) tensor; the states behind N are zero.
-    __device__ __forceinline__ void load_user(const float* row, int n0, int N, bool swap) {
-        if (N == 4 * NS) {
+    // A caller's (.., channels, N) tensor; the states behind N are zero.  `wide`: in packs, which wants N = 4 NS and the
+    // tensor on a 16-byte boundary.
+    __device__ __forceinline__ void load_user(const float* row, int n0, int N, bool swap, bool wide) {
+        if (wide) {
             load(row + n0, swap);
         } else {
 #pragma unroll
@@ -152,6 +154,8 @@ template <int NS> struct States {
             }
         }
     }
+    // States: the entry points have checked their addresses.
+    __device__ __forceinline__ void load_user(const float* row, int n0, int N, bool swap) { load_user(row, n0, N, swap, N == 4 * NS); }
     __device__ __forceinline__ void store_user(float* row, int n0, int N, bool swap) const {
         if (N == 4 * NS) {
             store(row + n0, swap);
@@ -372,7 +376,7 @@ template <int NS> __device__ __forceinline__ void load_rates(const ScanParams& p
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
         A2[ch].zero();
-        if (at.live[ch]) A2[ch].load_user(p.A + (int64_t)(at.c + ch) * p.states, at.q * NS, p.states, at.swap);
+        if (at.live[ch]) A2[ch].load_user(p.A + (int64_t)(at.c + ch) * p.states, at.q * NS, p.states, at.swap, p.wide_A != 0);
 #pragma unroll
         for (int i = 0; i < NS / 2; ++i) A2[ch].v[i] = mul2(A2[ch].v[i], F2(1.44269504f));
     }
@@ -1094,7 +1098,8 @@ __global__ void __launch_bounds__(4 * kStepChannels) scan_step_kernel(const Scan
         const int group = c / (p.channels / p.groups);
         States<NS> h, A;
         h.load_user(hp, n0, N);
-        A.load_user(p.A + (int64_t)c * N, n0, N);
+        if (p.wide_A) A.load_wide(p.A + (int64_t)c * N + n0);
+        else A.load_user(p.A + (int64_t)c * N, n0, N, false, false);
         const T* Bp = Bm + b * p.bs[0] + group * p.bs[2];
         const T* Cp = Cm + b * p.cs[0] + group * p.cs[2];
         xv = to_f<T>(x[b * p.xs[0] + c]);

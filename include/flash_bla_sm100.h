@@ -424,7 +424,7 @@ int fbla_causal_conv_step(const fbla_conv_problem *p, const void *x, const void 
  *   y[t,c] = (sum_n C[t,g,n] h[c,n] + D[c] x[t,c]) * z sigmoid(z),   g = c / (channels / groups)
  * x, dt, z, dy (batch, seq_len, channels) and B, C (batch, seq_len, groups, states) of `dtype`
  * with the given strides (elements), the last dimension contiguous; y, dx, ddt, dz, dB, dC
- * contiguous; A (channels, states), D, dt_bias (channels) and their gradients fp32.  States
+ * contiguous; A (channels, states), D, dt_bias (channels) and their gradients fp32, at any address.  States
  * (sequences, channels, states) fp32, 16-byte aligned.  D, z, dt_bias, initial_state, final_state,
  * d_final_state, d_initial_state, dD, d_dt_bias may be NULL.  checkpoints: fp32, 16-byte aligned,
  * fbla_selective_scan_checkpoint_floats() of them; NULL when no backward follows.  Packed

@@ -348,3 +348,32 @@ def test_a_second_derivative_is_refused():
     y = selective_scan(*(v[k] for k in NAMES[:8]), dt_softplus=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y, v["x"], dy.cuda(), create_graph=True)
+
+
+# ---- the address of A -----------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("N", [8, 16, 32, 7])
+def test_parameters_at_any_offset_of_a_flat_buffer(off, N):
+    """A, D and dt_bias as views of one buffer, as an optimizer that keeps its parameters flat has them."""
+    C, T = 24, 40
+    t, dy, df = inputs(15 + N, (2, T), C, 1, N, torch.float32, 2)
+    want = run(t, dy, df, True)
+    flat = torch.cat([torch.zeros(off)] + [t[k].flatten() for k in ("A", "D", "bias")]).cuda().requires_grad_()
+    at = [off, off + C * N, off + C * N + C, off + C * N + 2 * C]
+    A, D, bias = (flat[lo:hi] for lo, hi in zip(at, at[1:]))
+    A = A.view(C, N)
+    assert A.data_ptr() % 16 and A.is_contiguous()
+    v = {k: leaf(t[k]) for k in ("x", "dt", "B", "C", "z", "init")}
+    y, f = selective_scan(v["x"], v["dt"], A, v["B"], v["C"], D, v["z"], bias, dt_softplus=True, initial_state=v["init"],
+                          return_final_state=True)
+    torch.autograd.backward((y, f), (dy.cuda(), df.cuda()))
+    assert torch.equal(y, want["y"]) and torch.equal(f, want["final"])
+    assert torch.equal(flat.grad[off:], torch.cat([want[k].flatten() for k in ("dA", "dD", "dbias")]))
+    assert all(torch.equal(v[k].grad, want[g]) for k, g in zip(NAMES, GRADS) if k in v)
+    with torch.no_grad():
+        a = {k: cuda(x) if k in ("A", "D", "bias", "init") else x[:, 0].cuda() for k, x in t.items()}
+        ends = [a["init"].clone() for _ in range(2)]
+        ys = [selective_scan_step(a["x"], a["dt"], r, a["B"], a["C"], h, d, a["z"], b, dt_softplus=True)
+              for h, (r, d, b) in zip(ends, ((a["A"], a["D"], a["bias"]), (A, D, bias)))]
+    assert torch.equal(*ys) and torch.equal(*ends)
