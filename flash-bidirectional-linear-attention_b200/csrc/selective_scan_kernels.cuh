@@ -36,6 +36,7 @@ namespace scan {
 
 using fbla::seq::Pack;
 using fbla::seq::seq_of;
+using fbla::seq::ex2;
 using fbla::seq::F2;
 using fbla::seq::fma2;
 using fbla::seq::mul2;
@@ -387,6 +388,17 @@ template <int NS> __device__ __forceinline__ int64_t seg_at(const ScanParams& p,
     return (b * p.segs + seg) * p.channels + c;
 }
 
+// own + 2^x v, where 2^x is the decay of a whole segment and `near` the same in one product: far from 1 it can leave
+// fp32's range although its product with a state does not (e^128 times a state that is still zero; e^-128 times 1e30),
+// and is then applied in three factors, which reach from 2^-378 to 2^378; beyond, the product is out of range as well.
+// The factors themselves are neither zero nor infinite, so a state that is stays it, as it does token by token.  No
+// branch: with one, the next segments' loads wait for it (26 of them: 10 us).
+__device__ __forceinline__ float add_decayed(float x, float v, float own, float near) {
+    const float t = ex2(fminf(fmaxf(x * (1.f / 3.f), -126.f), 126.f));
+    const float far = fmaf(v * t * t, t, own);
+    return fabsf(x) > 126.f ? far : near;
+}
+
 // v <- own state of segment j + (its decay) v, for the lane's two channels
 template <int NS>
 __device__ __forceinline__ void add_segment(const ScanParams& p, const Place<NS>& at, int j, const float* seg_v, const float* seg_d,
@@ -399,8 +411,11 @@ __device__ __forceinline__ void add_segment(const ScanParams& p, const Place<NS>
         States<NS> own;
         own.load(seg_v + k * Tile<NS>::kNP + at.q * NS, at.swap);
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i)
-            v[ch].v[i] = sd == INFINITY ? own.v[i] : fma2(decay2(mul2(F2(sd), A2[ch].v[i])), v[ch].v[i], own.v[i]);
+        for (int i = 0; i < NS / 2; ++i) {
+            const F2 x = mul2(F2(sd), A2[ch].v[i]), w = v[ch].v[i], o = own.v[i], near = fma2(decay2(x), w, o);
+            const F2 r(add_decayed(x.x(), w.x(), o.x(), near.x()), add_decayed(x.y(), w.y(), o.y(), near.y()));
+            v[ch].v[i] = sd == INFINITY ? o : r;
+        }
     }
 }
 

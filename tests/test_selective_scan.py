@@ -377,3 +377,32 @@ def test_parameters_at_any_offset_of_a_flat_buffer(off, N):
         ys = [selective_scan_step(a["x"], a["dt"], r, a["B"], a["C"], h, d, a["z"], b, dt_softplus=True)
               for h, (r, d, b) in zip(ends, ((a["A"], a["D"], a["bias"]), (A, D, bias)))]
     assert torch.equal(*ys) and torch.equal(*ends)
+
+
+@gpu
+def test_segments_whose_total_decay_leaves_the_range():
+    """Three segments of 128 tokens with d A = 1 or -1: a whole segment's factor e^128 or e^-128 is beyond fp32 while
+    its product with the state (zero, or 1e30) is not; the same for what comes back from behind."""
+    T, C, N = 384, 64, 16
+    rn = randn(20)
+    up, down = slice(0, 32), slice(32, 64)
+    t = dict(x=torch.zeros(1, T, C), dt=torch.full((1, T, C), 0.125), A=torch.full((C, N), 8.0), B=rn(1, T, 1, N), C=rn(1, T, 1, N),
+             D=None, z=None, bias=None, init=torch.zeros(1, C, N))
+    dy, df = torch.zeros(1, T, C), torch.zeros(1, C, N)
+    t["A"][down] = -8.0
+    t["x"][:, 340:, up], dy[:, :40, up] = rn(1, 44, 32), rn(1, 40, 32)          # nothing before it grows, or behind it
+    t["init"][:, down], df[:, down] = rn(1, 32, N, scale=1e30), rn(1, 32, N, scale=1e30)
+    got = run(t, dy, df, False)
+    args = [t[k] for k in NAMES[:8]] + [False, t["init"], dy, df]
+    ref, major = Q.scan(*args), Q.scan(*args, absolute=True)
+    # As in compare(), the largest of its counts for all; beside it what underflow takes: values run down from 1e30 to
+    # nothing, a state, a product or a partial sum below 2^-126 is 0, so each loses up to that, times a factor |B|, |C| < 6
+    # or |A| = 8 at most, in sums of no more than T terms (N per y, dx and ddt, C per dB and dC, T per dA)
+    floor = 8 * T * 2.0 ** -126
+    for key in ("y", "final", "dx", "ddt", "dA", "dB", "dC", "dinit"):
+        err = (got[key].detach().cpu().double() - ref[key]).abs()
+        assert (err <= Q.bounds(ref[key], major[key], torch.float32, 2 * (8 * T + 8) + T + 32) + floor).all(), key
+    t["init"][0, 40, 5] = float("inf")
+    y = selective_scan(*(cuda(t[k]) for k in NAMES[:5]), initial_state=cuda(t["init"])).cpu()
+    rest = torch.arange(C) != 40
+    assert y[0, :, 40].isinf().all() and y[0, :, rest].isfinite().all()
