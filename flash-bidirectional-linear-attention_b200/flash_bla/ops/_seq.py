@@ -70,6 +70,11 @@ def call(fn, prob, like, *args):
         _C.check(fn(ctypes.byref(prob), *args, _C.stream_of(like)))
 
 
+# After a kernel has written a caller's state through its address: as torch's own operations in place do, tell autograd, so
+# that a backward pass which still needs the old state raises instead of using the new one (0.2 us).
+moved = torch.autograd.graph.increment_version
+
+
 def scratch(nbytes, like):
     """(tensor or None, bytes) from torch's caching allocator: a workspace of this call alone."""
     if nbytes < 0:

@@ -159,4 +159,5 @@ def causal_conv1d_step(
                           activation == "silu", 0, 0, 1, x.stride(0))
     S.call(_C.lib().fbla_causal_conv_step, prob, x, x.data_ptr(), weight.data_ptr(), _C.ptr(bias),
            state.data_ptr(), y.data_ptr())
+    S.moved(state)
     return y

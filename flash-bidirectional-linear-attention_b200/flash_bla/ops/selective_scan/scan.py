@@ -212,4 +212,5 @@ def selective_scan_step(
                           bs[0], 0, bs[1] if len(bs) == 3 else 0, cs[0], 0, cs[1] if len(cs) == 3 else 0)
     S.call(_C.lib().fbla_selective_scan_step, prob, x, x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
            _C.ptr(D), _C.ptr(z), _C.ptr(dt_bias), state.data_ptr(), y.data_ptr())
+    S.moved(state)
     return y

@@ -198,3 +198,41 @@ def test_on_another_stream_and_at_once():
                 got[i] = selective_scan(*sets[i])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("which", ["convolution", "scan"])
+def test_a_step_on_a_state_that_a_backward_pass_needs_is_noticed(which):
+    """The state of a call with gradients moved on by a token before its backward pass: an error, as of torch's own
+    operations in place, and no wrong gradient."""
+    B, T, C, N = 2, 12, 32, 16
+    rn = randn(9)
+    x, dt, A, Bm = rn(B, T, C).cuda(), rn(B, T, C).abs().cuda(), -torch.exp(rn(C, N)).cuda(), rn(B, T, N).cuda()
+    w = rn(C, 4).cuda().requires_grad_()
+    A.requires_grad_()
+    if which == "convolution":
+        state = rn(B, 3, C).cuda()
+        whole = lambda: causal_conv1d(x, w, activation="silu", initial_state=state)             # noqa: E731
+        step = lambda: causal_conv1d_step(x[:, 0], state, w)                                    # noqa: E731
+    else:
+        state = rn(B, C, N).cuda()
+        whole = lambda: selective_scan(x, dt, A, Bm, Bm, initial_state=state)                   # noqa: E731
+        step = lambda: selective_scan_step(x[:, 0], dt[:, 0], A, Bm[:, 0], Bm[:, 0], state)     # noqa: E731
+    y = whole()
+    before = state._version
+    with torch.no_grad():
+        step()
+    versions = state._version - before
+    assert versions == 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    y = whole()                         # in the other order nothing is in the way
+    y.sum().backward()
+    with torch.no_grad():
+        step()
+    with torch.inference_mode():        # a state made there has no version to move on
+        held = state.clone()
+        causal_conv1d_step(x[:, 0], held, w) if which == "convolution" else \
+            selective_scan_step(x[:, 0], dt[:, 0], A, Bm[:, 0], Bm[:, 0], held)
+    with torch.no_grad():
+        step()
+    assert torch.equal(held, state)
