@@ -3,6 +3,7 @@ short causal convolution, the selective scan)."""
 import ctypes
 
 import torch
+from torch.autograd import forward_ad as _fw
 
 from flash_bla import _C
 
@@ -46,7 +47,18 @@ def aligned(t):
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
 
 
+def is_dual(*tensors):
+    """Whether one of them carries a forward-mode tangent, which a kernel would drop without a word."""
+    if getattr(_fw, "_current_level", 0) < 0:           # no forward-mode level is active
+        return False
+    return any(isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def wants_grad(*tensors):
+    """Whether the call has to go through its autograd function.  A dual input does not ``require`` a gradient, but there
+    it raises, with gradients switched off too."""
+    if is_dual(*tensors):
+        return True
     for t in tensors:
         if t is not None and t.requires_grad:
             return torch.is_grad_enabled()
@@ -54,14 +66,19 @@ def wants_grad(*tensors):
 
 
 def refuse_grad(what, *tensors):
+    if is_dual(*tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
     if wants_grad(*tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
-def refuse_second_order(what):
-    """At the head of a backward pass: with ``create_graph=True`` its results would look like constants."""
+def refuse_second_order(what, *grads):
+    """At the head of a backward pass: with ``create_graph=True`` its results would look like constants, and to a
+    forward-mode level as well."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no second derivative: its backward pass cannot run with create_graph=True")
+    if is_dual(*grads):
+        raise RuntimeError(f"{what} has no second derivative: its backward pass has no forward-mode derivative")
 
 
 def call(fn, prob, like, *args):

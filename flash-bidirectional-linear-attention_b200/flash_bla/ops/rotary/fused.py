@@ -122,7 +122,7 @@ class RotaryFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        S.refuse_second_order("rotary_embedding")
+        S.refuse_second_order("rotary_embedding", dq, dk)
         freqs, positions, cu = ctx.saved_tensors
         offset, factor, interleaved, axes, dims = ctx.args
         dq = dq if ctx.needs_input_grad[0] else None

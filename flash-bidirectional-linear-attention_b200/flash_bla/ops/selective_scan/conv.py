@@ -65,7 +65,7 @@ class CausalConv1dFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dfinal):
-        S.refuse_second_order("causal_conv1d")
+        S.refuse_second_order("causal_conv1d", dy, dfinal)
         x, weight, bias, state, cu = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.dense(dfinal)

@@ -99,7 +99,7 @@ class SelectiveScanFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dfinal):
-        S.refuse_second_order("selective_scan")
+        S.refuse_second_order("selective_scan", dy, dfinal)
         x, dt, A, B, C, D, z, dt_bias, state, cu, ckpt = ctx.saved_tensors
         dy = torch.zeros_like(x) if dy is None else S.rows(dy)
         dfinal = S.aligned(S.dense(dfinal))

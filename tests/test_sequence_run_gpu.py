@@ -236,3 +236,32 @@ def test_a_step_on_a_state_that_a_backward_pass_needs_is_noticed(which):
     with torch.no_grad():
         step()
     assert torch.equal(held, state)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """No operator has a forward-mode derivative: a dual input raises, under no_grad too, and so does a dual gradient."""
+    fw = torch.autograd.forward_ad
+    rn = randn(10)
+    B, T, C, N = 2, 6, 16, 4
+    x, w, dt, A, Bm = rn(B, T, C).cuda(), rn(C, 4).cuda(), rn(B, T, C).abs().cuda(), -torch.exp(rn(C, N)).cuda(), rn(B, T, N).cuda()
+    q, f = rn(2, 3, 5, 8).cuda(), rotary_frequencies(8)[0]
+    hist, state = rn(B, 3, C).cuda(), rn(B, C, N).cuda()
+    calls = [(lambda v: rotary_embedding(v, None, f), q), (lambda v: rotary_embedding(q, v, f), q),
+             (lambda v: rotary_decoupled_la(v, q, q, f), q), (lambda v: causal_conv1d(v, w), x), (lambda v: causal_conv1d(x, v), w),
+             (lambda v: causal_conv1d(x, w, initial_state=v), hist), (lambda v: selective_scan(v, dt, A, Bm, Bm), x),
+             (lambda v: selective_scan(x, dt, v, Bm, Bm), A), (lambda v: selective_scan(x, dt, A, Bm, v), Bm),
+             (lambda v: selective_scan(x, dt, A, Bm, Bm, initial_state=v), state),
+             (lambda v: causal_conv1d_step(v, hist, w), x[:, 0]), (lambda v: causal_conv1d_step(x[:, 0], v, w), hist),
+             (lambda v: selective_scan_step(v, dt[:, 0], A, Bm[:, 0], Bm[:, 0], state), x[:, 0])]
+    with fw.dual_level():
+        for i, (call, v) in enumerate(calls):
+            call(v)                     # an active level alone changes nothing
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError, match="jvp|forward-mode"):
+                    call(fw.make_dual(v, torch.ones_like(v)))
+                    pytest.fail(f"call {i} went through")
+    for call, v in (calls[0], calls[3], calls[6]):
+        v = v.clone().requires_grad_()
+        y = call(v)
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, v, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
