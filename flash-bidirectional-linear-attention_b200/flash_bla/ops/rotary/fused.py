@@ -151,7 +151,7 @@ def rotary_embedding(
             `(total_tokens, H, D)`.  Read with any strides as long as the features are contiguous.
         k: keys of the same layout, dtype, batch, length and features (the number of heads may differ), or `None`.
         freqs: float64 `(P,)`, radians per position of each pair; the first `2 P <= D` features are
-            rotated, the others copied.  See `rotary_frequencies`.
+            rotated, the others copied.  They get no gradient and must not require one.  See `rotary_frequencies`.
         positions: int32 or int64 `(L,)` or `(B, L)`, packed `(total_tokens,)`; with `axes > 1` a last
             dimension of `axes` coordinates, and pair `i` turns with coordinate `i // (P / axes)`.
             `None`: `offset`, `offset + 1`, ... in every sequence.
@@ -183,6 +183,8 @@ def rotary_embedding(
         raise ValueError("q has no heads")
     if freqs.dtype != torch.float64 or freqs.dim() != 1:
         raise TypeError("freqs must be a float64 tensor of shape (pairs,)")
+    if S.wants_grad(freqs):
+        raise RuntimeError("freqs get no gradient: detach them, or call under torch.no_grad()")
     pairs = freqs.numel()
     if not 1 <= pairs <= q.shape[-1] // 2:
         raise ValueError(f"{pairs} pairs do not fit {q.shape[-1]} features")

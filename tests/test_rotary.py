@@ -96,6 +96,19 @@ def test_refusals_on_cpu():
     refused(ValueError, "int32", q=q[0], cu_seqlens=torch.tensor([0, 5]))
 
 
+def test_frequencies_that_want_a_gradient_are_refused():
+    """They get none: refused, where they would otherwise stay as they are without a word."""
+    q, f = torch.zeros(2, 3, 5, 8), freqs_of(4).requires_grad_()
+    with pytest.raises(RuntimeError, match="freqs"):
+        rotary_embedding(q, None, f)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="freqs"):
+        rotary_embedding(q, None, fw.make_dual(f.detach(), torch.ones(4, dtype=torch.float64)))
+    for frequencies in (f.detach(), f):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            rotary_embedding(q, None, frequencies)
+
+
 def test_library_refuses_without_a_device():
     import ctypes
     from flash_bla import _C
