@@ -680,6 +680,7 @@ int fbla_causal_conv_fwd(const fbla_conv_problem* p, const void* x, const void* 
     r.w = w;
     r.bias = bias;
     r.gs[0] = r.gs[1] = 0;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return with_width(p->width, [&](auto k) {
@@ -703,6 +704,7 @@ int fbla_causal_conv_bwd(const fbla_conv_problem* p, const void* x, const void* 
                         (long long)(workspace ? workspace_bytes : 0));
     r.w = w;
     r.bias = bias;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return with_width(p->width, [&](auto k) {
@@ -724,6 +726,7 @@ int fbla_causal_conv_step(const fbla_conv_problem* p, const void* x, const void*
     r.w = w;
     r.bias = bias;
     r.xs[1] = r.gs[0] = r.gs[1] = 0;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return with_width(p->width, [&](auto k) {

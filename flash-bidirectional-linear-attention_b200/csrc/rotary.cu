@@ -229,6 +229,7 @@ extern "C" int fbla_rotary(const fbla_rotary_problem* p, const void* q, const vo
     if (p->batch == 0 || p->seq_len == 0) return FBLA_OK;
     if (q == nullptr || q_out == nullptr) return api_fail(FBLA_ERR_INVALID, "q or q_out is NULL");
     if (p->heads_k > 0 && (k == nullptr || k_out == nullptr)) return api_fail(FBLA_ERR_INVALID, "k or k_out is NULL");
+    if (int rc = fbla::seq::check_device_status()) return rc;
     RotaryParams r;
     r.batch = p->batch;
     r.hq = p->heads_q;

@@ -152,6 +152,7 @@ int fbla_selective_scan_fwd(const fbla_scan_problem* p, const void* x, const voi
     ScanTensors a = {};
     a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z; a.init = initial_state; a.y = y; a.fin = final_state; a.ckpt = checkpoints;
     a.ws = (float*)workspace;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) { return Launcher<std::remove_pointer_t<decltype(t)>>::fwd(r, a, (cudaStream_t)stream); }),
                   "selective scan");
 }
@@ -179,6 +180,7 @@ int fbla_selective_scan_bwd(const fbla_scan_problem* p, const void* x, const voi
     a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z; a.dy = dy; a.init = initial_state; a.dfin = d_final_state;
     a.dx = dx; a.ddt = ddt; a.dB = dB; a.dC = dC; a.dz = dz; a.ckpt = const_cast<float*>(checkpoints);
     a.dA = dA; a.dD = dD; a.dbias = d_dt_bias; a.dinit = d_initial_state; a.ws = (float*)workspace;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) { return Launcher<std::remove_pointer_t<decltype(t)>>::bwd(r, a, (cudaStream_t)stream); }),
                   "selective scan backward");
 }
@@ -203,6 +205,7 @@ int fbla_selective_scan_step(const fbla_scan_problem* p, const void* x, const vo
     for (int i = 0; i < 3; i += 2) r.vec = r.vec && r.bs[i] % ns == 0 && r.cs[i] % ns == 0;
     ScanTensors a = {};
     a.x = x; a.dt = dt; a.B = B; a.C = C; a.z = z; a.fin = state; a.y = y;
+    if (int rc = fbla::seq::check_device_status()) return rc;
     return finish(with_type(p->dtype, [&](auto* t) { return Launcher<std::remove_pointer_t<decltype(t)>>::step(r, a, (cudaStream_t)stream); }),
                   "selective scan step");
 }

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "fbla_common.cuh"
+#include "tc_kernels.cuh"
 
 namespace fbla {
 namespace seq {
@@ -167,6 +168,15 @@ __device__ __forceinline__ SeqSpan seq_of(const int32_t* cu, int n, int64_t t) {
         r.hi = cu[a];
     }
     return r;
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+
+// Like every launching call: not after another one gave up a bounded wait, whose results may be what this one is given.
+inline int check_device_status() {
+    const int site = fbla::tc_device_status();
+    if (site == 0) return FBLA_OK;
+    return fbla::api_fail(FBLA_ERR_DEVICE, "a kernel gave up a bounded wait (site %d); results are invalid", site);
 }
 
 inline bool aligned_to(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0; }

@@ -160,3 +160,46 @@ def test_state_sum_kernel_gives_up_on_a_silent_peer_and_recovers():
     works_again()
     print("CHILD-OK")
     """)
+
+
+def test_sequence_operators_refuse_after_a_wait_gave_up():
+    """Like every launching call: inputs may be what the failed call left."""
+    _run("""
+    from flash_bla.ops.rotary.fused import rotary_embedding, rotary_frequencies
+    from flash_bla.ops.selective_scan.conv import causal_conv1d, causal_conv1d_step
+    from flash_bla.ops.selective_scan.scan import selective_scan, selective_scan_step
+    x, w, hist = torch.randn(1, 9, 8, device="cuda"), torch.randn(8, 4, device="cuda"), torch.zeros(1, 3, 8, device="cuda")
+    dt, A, Bm, h = x.abs(), -torch.ones(8, 4, device="cuda"), torch.randn(1, 9, 4, device="cuda"), torch.zeros(1, 8, 4, device="cuda")
+    freqs = rotary_frequencies(64)[0]
+    xg = x.clone().requires_grad_()
+    outs = [causal_conv1d(xg, w), selective_scan(xg, dt, A, Bm, Bm)]
+    calls = [lambda: rotary_embedding(q, k, freqs), lambda: causal_conv1d(x, w), lambda: causal_conv1d_step(x[:, 0], hist, w),
+             lambda: selective_scan(x, dt, A, Bm, Bm), lambda: selective_scan_step(x[:, 0], dt[:, 0], A, Bm[:, 0], Bm[:, 0], h)]
+    calls += [lambda y=y: torch.autograd.grad(y, xg, x, retain_graph=True) for y in outs]
+
+    def turned_away():
+        n = 0
+        for call in calls:
+            try:
+                call()
+            except RuntimeError as e:
+                n += "bounded wait" in str(e)
+        return n
+
+    assert turned_away() == 0
+    n = 4096
+    bufs = [torch.ones(n, device="cuda") for _ in range(2)]
+    flags = [torch.zeros(64, dtype=torch.int32, device="cuda") for _ in range(2)]
+    arr = ctypes.c_void_p * 2
+    out = torch.zeros(n, device="cuda")
+    _C.check(L.fbla_peer_state_sum(2, 0, arr(*[b.data_ptr() for b in bufs]), arr(*[f.data_ptr() for f in flags]), n, 1,
+                                   out.data_ptr(), _C.stream_of(out)))
+    torch.cuda.synchronize()
+    assert L.fbla_device_status() == 901
+    hist.zero_()
+    assert turned_away() == len(calls) and not hist.any()
+    L.fbla_clear_device_status()
+    assert turned_away() == 0
+    works_again()
+    print("CHILD-OK")
+    """)
