@@ -252,3 +252,29 @@ def test_many_short_sequences_and_no_token_at_all():
     got = run(x[:0], w, b, None, init[:3], dy[:0], df[:3], none)
     assert got["y"].shape == (0, C) and torch.equal(got["final"].cpu(), init[:3]) and torch.equal(got["dinit"].cpu(), df[:3])
     assert not got["dw"].any() and not got["db"].any()
+
+
+@gpu
+def test_backward_offsets_beyond_32_bits():
+    """More than 2^31 elements: gradients of the last tokens are what they are on their own.  dy is zero but for the first
+    and the last 50 tokens, so the filter's gradient is the sum of two short calls'."""
+    T, C, W, n = 1_060_000, 2048, 4, 50
+    g = torch.Generator("cuda").manual_seed(2)
+    x = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w = torch.randn(C, W, device="cuda", generator=g)
+    dy = torch.zeros_like(x)
+    for part in (dy[:, :n], dy[:, -n:]):
+        part.normal_(generator=g)
+
+    def grads(x, dy, state=None):
+        x, v = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = causal_conv1d(x, v, activation="silu", initial_state=state)
+        return torch.autograd.grad(y, (x, v), dy)
+
+    dx, dw = grads(x, dy)
+    tail, dw_tail = grads(x[:, -n:].clone(), dy[:, -n:].clone(), x[:, -n - W + 1:-n].clone())
+    head, dw_head = grads(x[:, :n].clone(), dy[:, :n].clone())
+    assert torch.equal(dx[:, -n:], tail) and torch.equal(dx[:, :n], head)
+    # 2 n terms g x, |g| at most 1.1 |dy|, each product and each sum rounded once, on both sides
+    size = 1.1 * (dy[0, :n].abs().float().sum(0) + dy[0, -n:].abs().float().sum(0)) * x.abs().max().float()
+    assert ((dw - dw_head - dw_tail).abs() <= 2 * (2 * n + 1) * 2.0 ** -24 * size[:, None]).all()

@@ -406,3 +406,35 @@ def test_segments_whose_total_decay_leaves_the_range():
     y = selective_scan(*(cuda(t[k]) for k in NAMES[:5]), initial_state=cuda(t["init"])).cpu()
     rest = torch.arange(C) != 40
     assert y[0, :, 40].isinf().all() and y[0, :, rest].isfinite().all()
+
+
+@gpu
+def test_backward_offsets_beyond_32_bits():
+    """More than 2^31 elements, 2^32 floats of checkpoints and 2^31 of sums over channels: gradients of the last tokens are
+    what they are on their own from the state before them.  exp(-0.5 * 0.1 * 6000) leaves nothing of what came before."""
+    T, C, N, n, back = 1_050_000, 2048, 32, 64, 6000
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    dt = torch.empty(1, T, C, dtype=torch.bfloat16, device="cuda").uniform_(0.01, 0.2, generator=g)
+    Bm, Cm = (torch.randn(1, T, N, device="cuda", generator=g).bfloat16() for _ in range(2))
+    A = -torch.rand(C, N, device="cuda", generator=g) - 0.5
+    dy = torch.zeros_like(x)
+    dy[:, -n:].normal_(generator=g)
+
+    def grads(*t):
+        *t, dy = (v.detach().requires_grad_() for v in t)
+        y = selective_scan(t[0], t[1], A, *t[2:])
+        return (y.detach(),) + torch.autograd.grad(y, t, dy.detach())
+
+    whole = [v[:, -n:].clone() for v in grads(x, dt, Bm, Cm, dy)]
+    short = [v[:, -n - back:].clone() for v in (x, dt, Bm, Cm, dy)]
+    alone = [v[:, -n:].float() for v in grads(*short)]
+    # the same sums with every term positive; ddt = sum A r + x sum G B has a negative part, and dx = d sum G B
+    size = [v[:, -n:] for v in grads(*(v.float() if v is short[1] else v.float().abs() for v in short))]
+    size[2] = 2 * short[0][:, -n:].float().abs() * size[1] / short[1][:, -n:].float() - size[2]
+    for what, k, a, b, m in zip(("y", "dx", "ddt", "dB", "dC"), (1, 0, 2, 0, 1), whole, alone, size):
+        # dx and dB take nothing from before: the same operations on the same numbers.  The others are sums from states
+        # formed in other segments: 8 roundings for each of the 400 tokens that matter on either side, twice that for a
+        # product with G, and one step of bf16 where the roundings fall apart
+        err = (a.float() - b).abs()
+        assert (err <= (2.0 ** -7 * b.abs() + 2 * k * 3200 * 2.0 ** -24 * m if k else torch.zeros_like(err))).all(), what
