@@ -14,8 +14,9 @@
 // gradient (3.5 TB/s); with one load in flight per thread 124 and 298, with a group's loads in registers, where the
 // compiler decides what is waited for together, 66 and 214.
 // Two channels share the packed fp32 instructions: in plain ones the arithmetic (W products per element forward,
-// 3 W + 1 backward, a sigmoid) takes as long as the memory.  The weight gradient is summed in registers over a thread's run, in shared memory over the runs of a
-// block, and then over the blocks by a kernel of its own: no atomics, the same bits on every run.
+// 3 W + 1 backward, a sigmoid) takes as long as the memory.  The weight gradient is summed in registers over a
+// thread's run, in shared memory over the runs of a block, and then over the blocks by a kernel of its own: no atomics,
+// the same bits on every run.
 #include <type_traits>
 
 #include "seq_common.cuh"

@@ -35,8 +35,9 @@ struct RotaryParams {
 };
 
 // Sine and cosine of an angle in turns, reduced to half a turn in 64 bits: adding and taking away 1.5 * 2^52 rounds
-// to the nearest integer.  fp32 results: to two units in the last place; 16-bit ones: the special function unit's,
-// 2^-21 absolute, far below their rounding (forming them otherwise costs more than a dozen heads' products).
+// to the nearest integer.  fp32 results: to two units in the last place; 16-bit ones: the special function unit's, off by
+// at most 2^-20 absolute (documented 2^-21.2 on [-pi, pi], and up to 5 2^-24 from rounding f and its product with 2 pi),
+// far below their rounding (forming them otherwise costs more than a dozen heads' products).
 template <typename T> __device__ __forceinline__ void sincos_turns(double turns, float& s, float& c) {
     const double whole = __dadd_rn(__dadd_rn(turns, 6755399441055744.0), -6755399441055744.0);
     const float f = (float)(turns - whole);

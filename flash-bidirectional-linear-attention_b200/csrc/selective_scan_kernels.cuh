@@ -266,7 +266,7 @@ template <typename T, int NS, bool VEC> struct Share {
     static_assert(2 * kRows == V, "a warp's rows, 32 channels at a time");
     Pack<T, V> v;
     // `base`: the tensor at this row of the batch; tokens tb .. of which those before `end` exist
-    __device__ __forceinline__ void fetch(const T* base, int64_t stride, const ScanParams& p, const Place<NS>& at, int64_t tb, int64_t end) {
+    __device__ __forceinline__ void fetch(const T* base, int64_t stride, const Place<NS>& at, int64_t tb, int64_t end) {
         if constexpr (VEC) {
             const int c = at.c0 + at.col();
             const int64_t t = tb + at.row();
@@ -286,7 +286,7 @@ template <typename T, int NS, bool VEC> struct Share {
             }
         }
     }
-    __device__ __forceinline__ void settle(const ScanParams& p, const Place<NS>& at, void* scratch) {
+    __device__ __forceinline__ void settle(const Place<NS>& at, void* scratch) {
         if constexpr (VEC) return;
         T* s = reinterpret_cast<T*>(scratch) + at.warp * kRows * kCB;
         __syncwarp();
@@ -299,7 +299,7 @@ template <typename T, int NS, bool VEC> struct Share {
 };
 // The way back; rows of `stride` elements.  All lanes of a warp take part.
 template <typename T, int NS, bool VEC>
-__device__ __forceinline__ void store_share(const float (&o)[Tile<NS>::kVPT], T* base, int64_t stride, const ScanParams& p, const Place<NS>& at,
+__device__ __forceinline__ void store_share(const float (&o)[Tile<NS>::kVPT], T* base, int64_t stride, const Place<NS>& at,
                                             int64_t tb, int64_t end, void* scratch) {
     using Sh = Share<T, NS, VEC>;
     constexpr int V = Sh::V;
@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
     Share<T, NS, VEC> px, pd;
     BCShare<T, NS> pB, pC;
     auto fetch = [&](int64_t tb) {
-        px.fetch(x + at.b * p.xs[0], p.xs[1], p, at, tb, t1);
-        pd.fetch(dt + at.b * p.ds[0], p.ds[1], p, at, tb, t1);
+        px.fetch(x + at.b * p.xs[0], p.xs[1], at, tb, t1);
+        pd.fetch(dt + at.b * p.ds[0], p.ds[1], at, tb, t1);
         pB.load(Bm, p.bs, p, at, tb, t1);
         if (!LOCAL) pC.load(Cm, p.cs, p, at, tb, t1);
     };
@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
         const bool marked = VARLEN && fill_marks(p, &sm.marks, tb, L::kTok, t1);
         bool ok = tb + row < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
-        px.settle(p, at, sm.scratch);
-        pd.settle(p, at, sm.scratch);
+        px.settle(at, sm.scratch);
+        pd.settle(at, sm.scratch);
         Share<T, NS, VEC> cx, cz;
         cx.v.zero();
         if (ok) cx = px;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
 
         if (tb + L::kTok < t1) fetch(tb + L::kTok);
         if (!LOCAL) {
-            if (z != nullptr) cz.fetch(z + at.b * p.zs[0], p.zs[1], p, at, tb, t1);
+            if (z != nullptr) cz.fetch(z + at.b * p.zs[0], p.zs[1], at, tb, t1);
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch)
                 if (ckpt != nullptr && at.live[ch])
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
         else work(std::false_type());
         __syncthreads();
         if (!LOCAL) {
-            if (z != nullptr) cz.settle(p, at, sm.scratch);
+            if (z != nullptr) cz.settle(at, sm.scratch);
             float out[V];
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
                 if (z != nullptr) out[i] *= cz.get(i) * fbla::seq::sigmoid<T>(cz.get(i));
                 if (!ok) out[i] = 0.f;
             }
-            store_share<T, NS, VEC>(out, y + at.b * p.len * p.channels, p.channels, p, at, tb, t1, sm.scratch);
+            store_share<T, NS, VEC>(out, y + at.b * p.len * p.channels, p.channels, at, tb, t1, sm.scratch);
         }
     }
 #pragma unroll
@@ -594,16 +594,16 @@ template <typename T, int NS, bool VEC> struct BwdShare {
     Share<T, NS, VEC> x, dt, z, dy;
     __device__ __forceinline__ void fetch(const ScanParams& p, const Place<NS>& at, const T* xp, const T* dtp, const T* zp, const T* dyp,
                                           int64_t tb, int64_t end) {
-        if (xp != nullptr) x.fetch(xp + at.b * p.xs[0], p.xs[1], p, at, tb, end);
-        dt.fetch(dtp + at.b * p.ds[0], p.ds[1], p, at, tb, end);
-        dy.fetch(dyp + at.b * p.gs[0], p.gs[1], p, at, tb, end);
-        if (zp != nullptr) z.fetch(zp + at.b * p.zs[0], p.zs[1], p, at, tb, end);
+        if (xp != nullptr) x.fetch(xp + at.b * p.xs[0], p.xs[1], at, tb, end);
+        dt.fetch(dtp + at.b * p.ds[0], p.ds[1], at, tb, end);
+        dy.fetch(dyp + at.b * p.gs[0], p.gs[1], at, tb, end);
+        if (zp != nullptr) z.fetch(zp + at.b * p.zs[0], p.zs[1], at, tb, end);
     }
-    __device__ __forceinline__ void settle(const ScanParams& p, const Place<NS>& at, bool with_x, bool gated, void* scratch) {
-        if (with_x) x.settle(p, at, scratch);
-        dt.settle(p, at, scratch);
-        dy.settle(p, at, scratch);
-        if (gated) z.settle(p, at, scratch);
+    __device__ __forceinline__ void settle(const Place<NS>& at, bool with_x, bool gated, void* scratch) {
+        if (with_x) x.settle(at, scratch);
+        dt.settle(at, scratch);
+        dy.settle(at, scratch);
+        if (gated) z.settle(at, scratch);
     }
     // e = dy silu(z)
     __device__ __forceinline__ float e(int i, bool gated) const {
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_bwd_local_kernel(const ScanP
         const bool marked = VARLEN && fill_marks(p, &sm.marks, tb, L::kTok, t1);
         bool ok = tb + row < t1;
         if (VARLEN) ok = ok && sm.marks.inside[row];
-        next.settle(p, at, false, z != nullptr, sm.scratch);
+        next.settle(at, false, z != nullptr, sm.scratch);
 #pragma unroll
         for (int i = 0; i < L::kVPT / 2; ++i) {
             const float2 bias = sm.bias[at.slot_of(i)];
@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             bc.template put<VARLEN>(sm.B[0], sm.marks, NS > 2 ? sm.B[1] : nullptr);
             bc.load(Cm, p.cs, p, at, tb, t1);
             bc.template put<VARLEN>(sm.C[0], sm.marks, NS > 2 ? sm.C[1] : nullptr);
-            in.settle(p, at, true, z != nullptr, scratch);
+            in.settle(at, true, z != nullptr, scratch);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
                 const int s = at.slot_of(i);
@@ -997,10 +997,10 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
         }
         if (!VEC || t < t1) {           // without packs all lanes of a warp take part in its loads and stores
             Share<T, NS, VEC> xv, dtv;
-            xv.fetch(x + at.b * p.xs[0], p.xs[1], p, at, tb, t1);
-            dtv.fetch(dt + at.b * p.ds[0], p.ds[1], p, at, tb, t1);
-            xv.settle(p, at, scratch);
-            dtv.settle(p, at, scratch);
+            xv.fetch(x + at.b * p.xs[0], p.xs[1], at, tb, t1);
+            dtv.fetch(dt + at.b * p.ds[0], p.ds[1], at, tb, t1);
+            xv.settle(at, scratch);
+            dtv.settle(at, scratch);
             float ox[V], od[V], oz[V];
 #pragma unroll
             for (int i = 0; i < V; i += 2) {
@@ -1027,9 +1027,9 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
                 sum = make_float2(sum.x + od[i], sum.y + od[i + 1]);
             }
             const int64_t o = at.b * p.len * p.channels;
-            store_share<T, NS, VEC>(ox, dx + o, p.channels, p, at, tb, t1, scratch);
-            store_share<T, NS, VEC>(od, ddt + o, p.channels, p, at, tb, t1, scratch);
-            if (z != nullptr) store_share<T, NS, VEC>(oz, dz + o, p.channels, p, at, tb, t1, scratch);
+            store_share<T, NS, VEC>(ox, dx + o, p.channels, at, tb, t1, scratch);
+            store_share<T, NS, VEC>(od, ddt + o, p.channels, at, tb, t1, scratch);
+            if (z != nullptr) store_share<T, NS, VEC>(oz, dz + o, p.channels, at, tb, t1, scratch);
         }
     }
     __syncthreads();

@@ -66,9 +66,9 @@ def wants_grad(*tensors):
 
 
 def refuse_grad(what, *tensors):
-    if is_dual(*tensors):
-        raise RuntimeError(f"{what} has no forward-mode derivative")
     if wants_grad(*tensors):
+        if is_dual(*tensors):
+            raise RuntimeError(f"{what} has no forward-mode derivative")
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
