@@ -11,9 +11,9 @@
 // Everything is fp32; a decay close to 1 is where an error of the exponential would add up over the steps that a
 // state remembers, so those come from a polynomial that is exact at 0 (see decay2()).
 // Measured at B8-T4096-C2048, 16 states, bf16: forward 692 us, backward 2022 us.  Forward, on an SM with three CTAs:
-// special function unit 58 % busy, multiply-add units 56 %, issue slots 62 % -- the three limits lie within a tenth
-// of one another, and more warps (four CTAs, 128 registers) or unrolling gave nothing.  The special function unit
-// alone (16 + 4 operations per token and channel, 16 per clock and SM) would take 290 us forward.
+// special function unit 58 % busy, multiply-add units 56 %, issue slots 62 %, 1.1 stall cycles of fixed latency per
+// issue: no unit is at its limit, and more warps (four CTAs, 128 registers) or unrolling gave nothing.  The special
+// function unit alone (16 + 4 operations per token and channel, 16 per clock and SM) would take 290 us forward.
 //
 // Layout: four lanes share two channels, each lane holding N/4 states of both in registers, so a warp owns 16
 // channels and a CTA of four warps 64; the tokens go by in tiles whose x, dt (turned into d and d x once per
