@@ -526,7 +526,8 @@ __global__ void __launch_bounds__(kThreads, 3) scan_fwd_kernel(const ScanParams 
                         const float d = ch ? v.z : v.x;
                         const F2 d2(d), dx2(ch ? v.w : v.y);
                         h[ch] = state_before<NS, MARKED>(p, at, sm.marks, tt + k, init, h[ch], ch);
-                        if (LOCAL) sum_d[ch] += MARKED && sm.marks.first[tt + k] >= 0 ? INFINITY : d;
+                        // (not added: what a sequence before it made of the sum ends here)
+                        if (LOCAL) sum_d[ch] = MARKED && sm.marks.first[tt + k] >= 0 ? INFINITY : sum_d[ch] + d;
                         F2 s2(0.f);
 #pragma unroll
                         for (int i = 0; i < NS / 2; ++i) {

@@ -438,3 +438,25 @@ def test_backward_offsets_beyond_32_bits():
         # product with G, and one step of bf16 where the roundings fall apart
         err = (a.float() - b).abs()
         assert (err <= (2.0 ** -7 * b.abs() + 2 * k * 3200 * 2.0 ** -24 * m if k else torch.zeros_like(err))).all(), what
+
+
+@gpu
+@pytest.mark.parametrize("bad", ["nan", "-inf"])
+@pytest.mark.parametrize("where", [30, 280, 310, 500])
+def test_a_step_size_that_is_no_number_stays_in_its_sequence(bad, where):
+    """Packed sequences over several segments (128 tokens each): a NaN or infinite step size in one of them, in the segment
+    in which the next one begins too, shows in no output and no gradient of the others."""
+    cu = [0, 20, 300, 305, 560, 900]
+    t, dy, df = inputs(30, (cu[-1],), 24, 1, 16, torch.float32, len(cu) - 1)
+    t["dt"], t["bias"] = t["dt"].abs() * 0.1, t["bias"].abs() * 0.01
+    lens = torch.tensor(cu, dtype=torch.int32)
+    want = run(t, dy, df, False, lens)
+    t["dt"][where] = float(bad)
+    got = run(t, dy, df, False, lens)
+    own = max(i for i, lo in enumerate(cu) if lo <= where)
+    for key in ("y", "dx", "ddt", "dB", "dC", "dz"):
+        for lo, hi in (z for i, z in enumerate(zip(cu, cu[1:])) if i != own):
+            assert torch.equal(got[key][lo:hi], want[key][lo:hi]), (key, lo)
+    rest = torch.arange(len(cu) - 1) != own
+    assert torch.equal(got["final"][rest], want["final"][rest]) and torch.equal(got["dinit"][rest], want["dinit"][rest])
+    assert not got["y"][where].isfinite().any()
