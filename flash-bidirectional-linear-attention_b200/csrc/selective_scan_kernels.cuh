@@ -994,6 +994,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(
             float s = 0.f;
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) s += sm.dbc[k][tt][w];
+            // behind the last sequence its state still stands, and may be infinite: 0 times it is not 0
+            if (VARLEN && !sm.marks.inside[tt]) s = 0.f;
             part_bc[((((int64_t)at.tile_in_group * p.batch + at.b) * p.len + tb + tt) * p.groups + at.group) * (2 * L::kNP) + w] = s;
         }
         if (!VEC || t < t1) {           // without packs all lanes of a warp take part in its loads and stores

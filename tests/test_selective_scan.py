@@ -460,3 +460,20 @@ def test_a_step_size_that_is_no_number_stays_in_its_sequence(bad, where):
     rest = torch.arange(len(cu) - 1) != own
     assert torch.equal(got["final"][rest], want["final"][rest]) and torch.equal(got["dinit"][rest], want["dinit"][rest])
     assert not got["y"][where].isfinite().any()
+
+
+@gpu
+@pytest.mark.parametrize("bad", ["x", "init", "dt"])
+@pytest.mark.parametrize("N", [8, 16, 30])
+def test_gradients_behind_the_last_sequence_stay_zero(bad, N):
+    """Its last state is still in the registers there, and 0 times an infinite one is not 0."""
+    cu = torch.tensor([0, 7, 40], dtype=torch.int32)
+    t, dy, df = inputs(31, (75,), 24, 1, N, torch.float32, 2)
+    if bad == "init":
+        t["init"][1, 3, 2] = float("inf")
+    else:
+        t[bad][38, 3] = float("nan")
+    got = run(t, dy, df, True, cu)
+    assert not got["y"][38:40].isfinite().all() and not got["dC"][38:40].isfinite().all()
+    for key in ("y", "dx", "ddt", "dB", "dC", "dz"):
+        assert not got[key][40:].any() and got[key][:7].isfinite().all(), key
